@@ -338,6 +338,67 @@ int ck_expert_bias_forward(void* y, int64_t y_stride, const void* bias, int64_t 
 int ck_expert_bias_backward(const void* dy, int64_t dy_stride, const int64_t* expert_offsets, void* d_bias,
                             int64_t d_bias_stride, int64_t num_rows, int64_t N, int64_t E, int dtype, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Balance loss, z-loss and per-expert counts of an MoE router (no counterpart in the reference, whose layer returns its
+ * router logits for the caller to put such a loss on).  With p the softmax and lse the log-sum-exp of a token's E logits,
+ * m the mask (NULL: every token counts), N = sum m, c_e the selections of expert e by counting tokens:
+ *   balance = E sum_e (c_e / (N k)) (sum_t m_t p_te / N)          z = sum_t m_t lse_t^2 / N
+ *   d logits = m p [ g_b E / N (f_e - sum_j f_j p_tj) + g_z 2 / N lse_t ],  f_e = c_e / (N k)
+ *   logits [tokens, E], rows `ld` elements apart; selected int64 [tokens, k] (ids outside [0, E) count nowhere); mask one
+ *   byte per token (non-zero counts).  Masked rows may hold anything; N = 0 gives zeros; a row of
+ *   nothing but -inf or the type's lowest value has no probabilities and no lse.  balance, z: one fp32 each; counts int32 [E]; stats int32 [2] (N, counted selections), read by the
+ *   backward.  balance_grad / z_grad: one fp32 each on the device, or NULL for zero.  d_logits dense [tokens, E].
+ * E <= 1024, 1 <= k <= E, tokens * k < 2^31.  Sums in fp32 per workgroup, in fp64 over them, in a fixed order.
+ * ------------------------------------------------------------------------------------------- */
+int64_t ck_moe_balance_loss_workspace_size(int64_t tokens, int64_t E);
+int ck_moe_balance_loss_forward(const void* logits, int64_t ld, const int64_t* selected, const void* mask, float* balance,
+                                float* z, int* counts, int* stats, void* workspace, int64_t workspace_bytes,
+                                int64_t tokens, int64_t E, int64_t k, int dtype, void* stream);
+int ck_moe_balance_loss_backward(const void* logits, int64_t ld, const void* mask, const int* counts, const int* stats,
+                                 const float* balance_grad, const float* z_grad, void* d_logits, int64_t tokens, int64_t E,
+                                 int64_t k, int dtype, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Activations kept in 8 bits between forward and backward (no counterpart in the reference): MXINT8 of the OCP
+ * microscaling formats.  A block is 32 consecutive elements of a row, the last one of a row may be shorter; it has one
+ * scale byte b and int8 codes q in [-127, 127], element = q * 2^(b - 133).  b is the smallest exponent (7 .. 254) for
+ * which the block's largest magnitude rounds to at most 127 steps; rounding is to nearest, ties to even; b = 255 marks a
+ * block with a NaN or an infinity, which stands for NaNs.
+ *   codes: H bytes a row, scales: ceil(H / 32) bytes a row (dense unless a stride is passed)
+ * ck_mx8_quantize    x [rows, H] -> codes, scales
+ * ck_mx8_dequantize  output row r = kept row r, or kept row index[r] / fan (index int64 [rows]; a row outside
+ *                    [0, source_rows) becomes zeros).  A value beyond fp16's range becomes its largest finite number.
+ * ck_swiglu_forward_mx8 / _backward_mx8
+ *                    y = up * gate * sigmoid(gate), with gate and up also written in 8 bits; the gradients from those.
+ *                    Rows of gate, up and their gradients are `ldx` elements apart (two tensors, or the halves of one),
+ *                    codes `ldc` and scales `lds` bytes.  activation (or NULL): y recomputed from the kept inputs.
+ * ck_rmsnorm_forward_mx8 / _backward_mx8
+ *                    ck_rmsnorm_forward (residual NULL) or ck_residual_rmsnorm_forward with the normalised row's input
+ *                    also written in 8 bits; rstd fp32 [B] is always written.  Backward: x_grad and weight_grad from
+ *                    the kept rows and rstd; sum_grad (or NULL) is added to x_grad before it is rounded.  weight_grad
+ *                    is summed through `workspace` without atomics.
+ * ck_moe_combine_backward_gates_mx8
+ *                    ck_moe_combine_backward_gates with the expert outputs [tokens, k, H] in 8 bits.
+ * rows * 4 * ceil(H / 32) < 2^31 for the element-wise ones, H <= 65536 and B < 2^31 for RMSNorm.
+ * ------------------------------------------------------------------------------------------- */
+int ck_mx8_quantize(const void* x, void* codes, void* scales, int64_t rows, int64_t H, int dtype, void* stream);
+int ck_mx8_dequantize(const void* codes, const void* scales, const int64_t* index, int64_t fan, int64_t source_rows,
+                      void* output, int64_t rows, int64_t H, int dtype, void* stream);
+int ck_swiglu_forward_mx8(const void* gate, const void* up, int64_t ldx, void* output, void* gate_codes, void* up_codes,
+                          int64_t ldc, void* gate_scales, void* up_scales, int64_t lds, int64_t rows, int64_t H, int dtype,
+                          void* stream);
+int ck_swiglu_backward_mx8(const void* gate_codes, const void* up_codes, int64_t ldc, const void* gate_scales,
+                           const void* up_scales, int64_t lds, const void* output_grad, void* gate_grad, void* up_grad,
+                           int64_t ldx, void* activation, int64_t rows, int64_t H, int dtype, void* stream);
+int ck_rmsnorm_forward_mx8(const void* x, const void* residual, const void* weight, void* output, void* residual_out,
+                           void* codes, void* scales, float* rstd, int64_t B, int64_t H, float eps, int dtype, void* stream);
+int64_t ck_rmsnorm_backward_mx8_workspace_size(int64_t B, int64_t H);
+int ck_rmsnorm_backward_mx8(const void* codes, const void* scales, const void* weight, const void* output_grad,
+                            const float* rstd, const void* sum_grad, void* x_grad, void* weight_grad, void* workspace,
+                            int64_t workspace_bytes, int64_t B, int64_t H, int dtype, void* stream);
+int ck_moe_combine_backward_gates_mx8(const void* codes, const void* scales, const void* grad_out, void* d_gates,
+                                      int64_t tokens, int64_t k, int64_t H, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

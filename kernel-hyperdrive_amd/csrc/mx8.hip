@@ -1,0 +1,411 @@
+// Activations in 8 bits (ck_mx8.h) for gfx950: writing and reading them, SwiGLU forward with its inputs kept in 8 bits and
+// its backward from them, and the routing weights' gradient from expert outputs kept in 8 bits.
+// HBM-bound streaming kernels in the manner of swiglu.hip: a lane moves pieces of eight elements, several in flight, fp32
+// math, one rounding on store.
+#include "ck_mx8.h"
+
+namespace ck {
+
+constexpr int kMxThreads = 256;
+constexpr int kMxUnroll = 4;  // pieces per lane
+
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kMxThreads)
+    mx8_quantize_kernel(const typename T::storage_t* __restrict__ x, int8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                        MxShape shape) {
+    constexpr bool VEC = MODE != kMxAny;
+    const int64_t blocks = shape.per_row / kMxQuad;
+    const uint32_t base = blockIdx.x * (kMxThreads * kMxUnroll) + threadIdx.x;
+    Piece<T> in[kMxUnroll];
+#pragma unroll
+    for (int i = 0; i < kMxUnroll; ++i) {
+        const uint32_t p = base + i * kMxThreads;
+        const MxAt a = mx_at<MODE>(shape, p);
+        if (mx_has<MODE>(shape, p, a)) in[i] = load_piece<T, VEC>(x + a.row * shape.h + a.col, a.n);
+        else in[i].clear();
+    }
+#pragma unroll
+    for (int i = 0; i < kMxUnroll; ++i) {
+        const uint32_t p = base + i * kMxThreads;
+        const MxAt a = mx_at<MODE>(shape, p);
+        float v[kMxPiece];
+#pragma unroll
+        for (int j = 0; j < kMxPiece; ++j) v[j] = in[i].up(j);
+        uint32_t scale;
+        const MxCodes c = mx_encode(v, scale);
+        if (mx_has<MODE>(shape, p, a)) {
+            store_codes<VEC>(c, codes + a.row * shape.h + a.col, a.n);
+            if (threadIdx.x % kMxQuad == 0) scales[a.row * blocks + a.block] = (uint8_t)scale;
+        }
+    }
+}
+
+// What a kept value becomes in its storage type: itself, but that a block near fp16's end may stand for a value beyond it
+// (65504 is kept as 64 steps of 1024), which becomes the largest finite number.
+template <typename T>
+__device__ __forceinline__ float mx_limit(float v) {
+    return v;
+}
+template <>
+__device__ __forceinline__ float mx_limit<F16>(float v) {
+    return v > 65504.f ? 65504.f : (v < -65504.f ? -65504.f : v);  // (a NaN fails both comparisons)
+}
+
+// out row r is row (index != NULL ? index[r] / fan : r) of the kept matrix; rows outside it become zeros
+template <typename T, int MODE, bool GATHER>
+__global__ void __launch_bounds__(kMxThreads)
+    mx8_dequantize_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                          const int64_t* __restrict__ index, int64_t fan, int64_t source_rows,
+                          typename T::storage_t* __restrict__ out, MxShape shape) {
+    constexpr bool VEC = MODE != kMxAny;
+    const int64_t blocks = shape.per_row / kMxQuad;
+    const uint32_t base = blockIdx.x * (kMxThreads * kMxUnroll) + threadIdx.x;
+    MxCodes in[kMxUnroll];
+    uint32_t scale[kMxUnroll];
+#pragma unroll
+    for (int i = 0; i < kMxUnroll; ++i) {
+        const uint32_t p = base + i * kMxThreads;
+        const MxAt a = mx_at<MODE>(shape, p);
+        in[i].w[0] = in[i].w[1] = 0;
+        scale[i] = 7;
+        if (mx_has<MODE>(shape, p, a)) {
+            const int64_t row = GATHER ? index[a.row] / fan : a.row;
+            if (!GATHER || (row >= 0 && row < source_rows)) {
+                in[i] = load_codes<VEC>(codes + row * shape.h + a.col, a.n);
+                scale[i] = scales[row * blocks + a.block];
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kMxUnroll; ++i) {
+        const uint32_t p = base + i * kMxThreads;
+        const MxAt a = mx_at<MODE>(shape, p);
+        float v[kMxPiece];
+        mx_decode(in[i], mx_step(scale[i]), v);
+        if (mx_has<MODE>(shape, p, a)) {
+            Piece<T> o;
+#pragma unroll
+            for (int j = 0; j < kMxPiece; ++j) {
+                o.put(j, mx_limit<T>(v[j]));
+            }
+            store_piece<T, VEC>(o, out + a.row * shape.h + a.col, a.n);
+        }
+    }
+}
+
+// ---- SwiGLU ----------------------------------------------------------------------------------------------------------
+// gate, up: rows of h elements ld apart (one tensor each, or the halves of one); codes and scales likewise, with distances
+// of their own.
+struct MxStrides {
+    int64_t x, codes, scales;
+};
+
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kMxThreads)
+    swiglu_fwd_mx8_kernel(const typename T::storage_t* __restrict__ gate, const typename T::storage_t* __restrict__ up,
+                          typename T::storage_t* __restrict__ out, int8_t* __restrict__ gate_codes,
+                          int8_t* __restrict__ up_codes, uint8_t* __restrict__ gate_scales, uint8_t* __restrict__ up_scales,
+                          MxStrides ld, MxShape shape) {
+    constexpr bool VEC = MODE != kMxAny;
+    constexpr int kUnroll = 2;  // two tensors: as many bytes in flight as the one-tensor kernels
+    const uint32_t base = blockIdx.x * (kMxThreads * kUnroll) + threadIdx.x;
+    Piece<T> g[kUnroll], u[kUnroll];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+        const uint32_t p = base + i * kMxThreads;
+        const MxAt a = mx_at<MODE>(shape, p);
+        if (mx_has<MODE>(shape, p, a)) {
+            g[i] = load_piece<T, VEC>(gate + a.row * ld.x + a.col, a.n);
+            u[i] = load_piece<T, VEC>(up + a.row * ld.x + a.col, a.n);
+        } else {
+            g[i].clear();
+            u[i].clear();
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+        const uint32_t p = base + i * kMxThreads;
+        const MxAt a = mx_at<MODE>(shape, p);
+        float gv[kMxPiece], uv[kMxPiece];
+        Piece<T> y;
+#pragma unroll
+        for (int j = 0; j < kMxPiece; ++j) {
+            gv[j] = g[i].up(j);
+            uv[j] = u[i].up(j);
+            y.put(j, swiglu_fwd_1<T>(gv[j], uv[j]));
+        }
+        uint32_t gs, us;
+        const MxCodes gc = mx_encode(gv, gs), uc = mx_encode(uv, us);
+        if (mx_has<MODE>(shape, p, a)) {
+            store_piece<T, VEC>(y, out + a.row * shape.h + a.col, a.n);
+            store_codes<VEC>(gc, gate_codes + a.row * ld.codes + a.col, a.n);
+            store_codes<VEC>(uc, up_codes + a.row * ld.codes + a.col, a.n);
+            if (threadIdx.x % kMxQuad == 0) {
+                gate_scales[a.row * ld.scales + a.block] = (uint8_t)gs;
+                up_scales[a.row * ld.scales + a.block] = (uint8_t)us;
+            }
+        }
+    }
+}
+
+// sigmoid(x) with its relative accuracy kept on both sides (for x < 0 it is the exponential itself that carries it)
+template <typename T>
+__device__ __forceinline__ float mx_sigmoid(float x) {
+    return sigmoidf_<T>(x);
+}
+template <>
+__device__ __forceinline__ float mx_sigmoid<F32>(float x) {
+    const float e = expf(-fabsf(x));
+    const float r = 1.0f / (1.0f + e);
+    return x >= 0.f ? r : e * r;
+}
+
+// ACT: also writes the activation the kept inputs give (for the next product's weight gradient)
+template <typename T, int MODE, bool ACT>
+__global__ void __launch_bounds__(kMxThreads)
+    swiglu_bwd_mx8_kernel(const int8_t* __restrict__ gate_codes, const int8_t* __restrict__ up_codes,
+                          const uint8_t* __restrict__ gate_scales, const uint8_t* __restrict__ up_scales,
+                          const typename T::storage_t* __restrict__ dy, typename T::storage_t* __restrict__ dgate,
+                          typename T::storage_t* __restrict__ dup, typename T::storage_t* __restrict__ act, MxStrides ld,
+                          MxShape shape) {
+    constexpr bool VEC = MODE != kMxAny;
+    constexpr int kUnroll = 2;
+    const uint32_t base = blockIdx.x * (kMxThreads * kUnroll) + threadIdx.x;
+    MxCodes gc[kUnroll], uc[kUnroll];
+    uint32_t gs[kUnroll], us[kUnroll];
+    Piece<T> d[kUnroll];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+        const uint32_t p = base + i * kMxThreads;
+        const MxAt a = mx_at<MODE>(shape, p);
+        if (mx_has<MODE>(shape, p, a)) {
+            gc[i] = load_codes<VEC>(gate_codes + a.row * ld.codes + a.col, a.n);
+            uc[i] = load_codes<VEC>(up_codes + a.row * ld.codes + a.col, a.n);
+            gs[i] = gate_scales[a.row * ld.scales + a.block];
+            us[i] = up_scales[a.row * ld.scales + a.block];
+            d[i] = load_piece<T, VEC>(dy + a.row * shape.h + a.col, a.n);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+        const uint32_t p = base + i * kMxThreads;
+        const MxAt a = mx_at<MODE>(shape, p);
+        if (mx_has<MODE>(shape, p, a)) {
+            float g[kMxPiece], u[kMxPiece];
+            mx_decode(gc[i], mx_step(gs[i]), g);
+            mx_decode(uc[i], mx_step(us[i]), u);
+            Piece<T> og, ou, oa;
+#pragma unroll
+            for (int j = 0; j < kMxPiece; ++j) {
+                const float dy1 = d[i].up(j), s = mx_sigmoid<T>(g[j]), gs = g[j] * s;
+                og.put(j, dy1 * u[j] * (s + gs * (1.0f - s)));
+                ou.put(j, dy1 * gs);
+                if (ACT) oa.put(j, u[j] * gs);
+            }
+            store_piece<T, VEC>(og, dgate + a.row * ld.x + a.col, a.n);
+            store_piece<T, VEC>(ou, dup + a.row * ld.x + a.col, a.n);
+            if (ACT) store_piece<T, VEC>(oa, act + a.row * shape.h + a.col, a.n);
+        }
+    }
+}
+
+// ---- routing weights' gradient: d_gates[t, s] = <expert output s of token t (kept in 8 bits), grad_out[t]> ------------------
+// one wavefront per token, as in moe_combine.hip
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256)
+    combine_bwd_gates_mx8_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                                 const typename T::storage_t* __restrict__ grad_out,
+                                 typename T::storage_t* __restrict__ d_gates, int64_t tokens, int k, int64_t H) {
+    const int64_t t = (int64_t)blockIdx.x * 4 + threadIdx.x / CK_WAVE;
+    if (t >= tokens) return;
+    const int lane = lane_id();
+    const int64_t blocks = (H + kMxBlock - 1) / kMxBlock;
+    const int64_t pieces = (H + kMxPiece - 1) / kMxPiece;
+    const typename T::storage_t* dy = grad_out + t * H;
+    for (int s = 0; s < k; ++s) {
+        const int64_t row = t * k + s;
+        float acc = 0.f;
+        for (int64_t p = lane; p < pieces; p += CK_WAVE) {
+            const int64_t left = H - p * kMxPiece;
+            const int n = left >= kMxPiece ? kMxPiece : (int)left;
+            const MxCodes c = load_codes<VEC>(codes + row * H + p * kMxPiece, n);
+            const float step = mx_step(scales[row * blocks + p / kMxQuad]);
+            const Piece<T> b = load_piece<T, VEC, false>(dy + p * kMxPiece, n);  // (re-read per slot: stays in the caches)
+            float v[kMxPiece];
+            mx_decode(c, step, v);
+#pragma unroll
+            for (int j = 0; j < kMxPiece; ++j)
+                if (VEC || j < n) acc += v[j] * b.up(j);
+        }
+        acc = wave_sum(acc);
+        if (lane == 0) d_gates[row] = T::down(acc);
+    }
+}
+
+}  // namespace ck
+
+// ---- host side ---------------------------------------------------------------------------------------------------------
+static bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
+
+// kMxRows wherever every row starts on a whole packet, kMxFlat where the rows are one run besides
+static int mx_mode(int64_t h, bool aligned, bool dense) {
+    if (!aligned || h % ck::kMxPiece != 0) return ck::kMxAny;
+    return dense && h % ck::kMxBlock == 0 ? ck::kMxFlat : ck::kMxRows;
+}
+
+#define CK_MX_MODE(mode, ...)                              \
+    if ((mode) == ck::kMxFlat) {                           \
+        constexpr int MODE = ck::kMxFlat;                  \
+        __VA_ARGS__;                                       \
+    } else if ((mode) == ck::kMxRows) {                    \
+        constexpr int MODE = ck::kMxRows;                  \
+        __VA_ARGS__;                                       \
+    } else {                                               \
+        constexpr int MODE = ck::kMxAny;                   \
+        __VA_ARGS__;                                       \
+    }
+
+static dim3 mx_grid(const ck::MxShape& s, int unroll) {
+    return dim3((unsigned)ck_ceil_div((int64_t)s.total, (int64_t)ck::kMxThreads * unroll));
+}
+static bool mx_dtype(int dtype) { return dtype == CK_F32 || dtype == CK_F16 || dtype == CK_BF16; }
+
+extern "C" int ck_mx8_quantize(const void* x, void* codes, void* scales, int64_t rows, int64_t H, int dtype, void* stream) {
+    if (rows < 0 || H < 0) return CK_ERR_SHAPE;
+    if (!mx_dtype(dtype)) return CK_ERR_DTYPE;
+    if (rows == 0 || H == 0) return CK_OK;
+    if (!x || !codes || !scales) return CK_ERR_NULL;
+    if (!ck_aligned_elem(x, dtype)) return CK_ERR_ALIGN;
+    ck::MxShape shape;
+    if (!ck::mx_shape(rows, H, &shape)) return CK_ERR_SHAPE;
+    hipStream_t s = (hipStream_t)stream;
+    const int mode = mx_mode(H, ck_aligned16(x) && aligned8(codes), true);
+    CK_DISPATCH_DTYPE(dtype, {
+        typedef typename T::storage_t S;
+        CK_MX_MODE(mode, {
+            hipLaunchKernelGGL((ck::mx8_quantize_kernel<T, MODE>), mx_grid(shape, ck::kMxUnroll), dim3(ck::kMxThreads), 0, s,
+                               (const S*)x, (int8_t*)codes, (uint8_t*)scales, shape);
+        });
+    });
+    return ck_launch_status();
+}
+
+extern "C" int ck_mx8_dequantize(const void* codes, const void* scales, const int64_t* index, int64_t fan,
+                                 int64_t source_rows, void* output, int64_t rows, int64_t H, int dtype, void* stream) {
+    if (rows < 0 || H < 0 || fan < 1 || source_rows < 0 || (!index && source_rows < rows)) return CK_ERR_SHAPE;
+    if (!mx_dtype(dtype)) return CK_ERR_DTYPE;
+    if (rows == 0 || H == 0) return CK_OK;
+    if (!output || (source_rows > 0 && (!codes || !scales))) return CK_ERR_NULL;
+    if (!ck_aligned_elem(output, dtype)) return CK_ERR_ALIGN;
+    ck::MxShape shape;
+    if (!ck::mx_shape(rows, H, &shape)) return CK_ERR_SHAPE;
+    hipStream_t s = (hipStream_t)stream;
+    const int mode = mx_mode(H, ck_aligned16(output) && aligned8(codes), index == nullptr);
+    CK_DISPATCH_DTYPE(dtype, {
+        typedef typename T::storage_t S;
+        if (index == nullptr) {
+            CK_MX_MODE(mode, {
+                hipLaunchKernelGGL((ck::mx8_dequantize_kernel<T, MODE, false>), mx_grid(shape, ck::kMxUnroll),
+                                   dim3(ck::kMxThreads), 0, s, (const int8_t*)codes, (const uint8_t*)scales, index, fan,
+                                   source_rows, (S*)output, shape);
+            });
+        } else if (mode == ck::kMxRows) {
+            hipLaunchKernelGGL((ck::mx8_dequantize_kernel<T, ck::kMxRows, true>), mx_grid(shape, ck::kMxUnroll),
+                               dim3(ck::kMxThreads), 0, s, (const int8_t*)codes, (const uint8_t*)scales, index, fan,
+                               source_rows, (S*)output, shape);
+        } else {
+            hipLaunchKernelGGL((ck::mx8_dequantize_kernel<T, ck::kMxAny, true>), mx_grid(shape, ck::kMxUnroll),
+                               dim3(ck::kMxThreads), 0, s, (const int8_t*)codes, (const uint8_t*)scales, index, fan,
+                               source_rows, (S*)output, shape);
+        }
+    });
+    return ck_launch_status();
+}
+
+extern "C" int ck_swiglu_forward_mx8(const void* gate, const void* up, int64_t ldx, void* output, void* gate_codes,
+                                     void* up_codes, int64_t ldc, void* gate_scales, void* up_scales, int64_t lds,
+                                     int64_t rows, int64_t H, int dtype, void* stream) {
+    if (rows < 0 || H < 0 || ldx < H || ldc < H || lds < ck::mx_blocks(H)) return CK_ERR_SHAPE;
+    if (!mx_dtype(dtype)) return CK_ERR_DTYPE;
+    if (rows == 0 || H == 0) return CK_OK;
+    if (!gate || !up || !output || !gate_codes || !up_codes || !gate_scales || !up_scales) return CK_ERR_NULL;
+    if (!ck_aligned_elem(gate, dtype) || !ck_aligned_elem(up, dtype) || !ck_aligned_elem(output, dtype)) return CK_ERR_ALIGN;
+    ck::MxShape shape;
+    if (!ck::mx_shape(rows, H, &shape)) return CK_ERR_SHAPE;
+    hipStream_t s = (hipStream_t)stream;
+    const bool aligned = ck_aligned16(gate) && ck_aligned16(up) && ck_aligned16(output) && aligned8(gate_codes) &&
+                         aligned8(up_codes) && ldx % ck::kMxPiece == 0 && ldc % ck::kMxPiece == 0;
+    const bool dense = ldx == H && ldc == H && lds == ck::mx_blocks(H);
+    const int mode = mx_mode(H, aligned, dense);
+    const ck::MxStrides ld = {ldx, ldc, lds};
+    CK_DISPATCH_DTYPE(dtype, {
+        typedef typename T::storage_t S;
+        CK_MX_MODE(mode, {
+            hipLaunchKernelGGL((ck::swiglu_fwd_mx8_kernel<T, MODE>), mx_grid(shape, 2), dim3(ck::kMxThreads), 0, s,
+                               (const S*)gate, (const S*)up, (S*)output, (int8_t*)gate_codes, (int8_t*)up_codes,
+                               (uint8_t*)gate_scales, (uint8_t*)up_scales, ld, shape);
+        });
+    });
+    return ck_launch_status();
+}
+
+extern "C" int ck_swiglu_backward_mx8(const void* gate_codes, const void* up_codes, int64_t ldc, const void* gate_scales,
+                                      const void* up_scales, int64_t lds, const void* output_grad, void* gate_grad,
+                                      void* up_grad, int64_t ldx, void* activation, int64_t rows, int64_t H, int dtype,
+                                      void* stream) {
+    if (rows < 0 || H < 0 || ldx < H || ldc < H || lds < ck::mx_blocks(H)) return CK_ERR_SHAPE;
+    if (!mx_dtype(dtype)) return CK_ERR_DTYPE;
+    if (rows == 0 || H == 0) return CK_OK;
+    if (!gate_codes || !up_codes || !gate_scales || !up_scales || !output_grad || !gate_grad || !up_grad) return CK_ERR_NULL;
+    if (!ck_aligned_elem(output_grad, dtype) || !ck_aligned_elem(gate_grad, dtype) || !ck_aligned_elem(up_grad, dtype) ||
+        !ck_aligned_elem(activation, dtype))
+        return CK_ERR_ALIGN;
+    ck::MxShape shape;
+    if (!ck::mx_shape(rows, H, &shape)) return CK_ERR_SHAPE;
+    hipStream_t s = (hipStream_t)stream;
+    const bool aligned = ck_aligned16(output_grad) && ck_aligned16(gate_grad) && ck_aligned16(up_grad) &&
+                         ck_aligned16(activation) && aligned8(gate_codes) && aligned8(up_codes) &&
+                         ldx % ck::kMxPiece == 0 && ldc % ck::kMxPiece == 0;
+    const bool dense = ldx == H && ldc == H && lds == ck::mx_blocks(H);
+    const int mode = mx_mode(H, aligned, dense);
+    const ck::MxStrides ld = {ldx, ldc, lds};
+    CK_DISPATCH_DTYPE(dtype, {
+        typedef typename T::storage_t S;
+        CK_MX_MODE(mode, {
+            if (activation)
+                hipLaunchKernelGGL((ck::swiglu_bwd_mx8_kernel<T, MODE, true>), mx_grid(shape, 2), dim3(ck::kMxThreads), 0, s,
+                                   (const int8_t*)gate_codes, (const int8_t*)up_codes, (const uint8_t*)gate_scales,
+                                   (const uint8_t*)up_scales, (const S*)output_grad, (S*)gate_grad, (S*)up_grad,
+                                   (S*)activation, ld, shape);
+            else
+                hipLaunchKernelGGL((ck::swiglu_bwd_mx8_kernel<T, MODE, false>), mx_grid(shape, 2), dim3(ck::kMxThreads), 0,
+                                   s, (const int8_t*)gate_codes, (const int8_t*)up_codes, (const uint8_t*)gate_scales,
+                                   (const uint8_t*)up_scales, (const S*)output_grad, (S*)gate_grad, (S*)up_grad,
+                                   (S*)nullptr, ld, shape);
+        });
+    });
+    return ck_launch_status();
+}
+
+extern "C" int ck_moe_combine_backward_gates_mx8(const void* codes, const void* scales, const void* grad_out, void* d_gates,
+                                                 int64_t tokens, int64_t k, int64_t H, int dtype, void* stream) {
+    if (tokens < 0 || k <= 0 || H < 0 || k > 0x7fffffff) return CK_ERR_SHAPE;
+    if (!mx_dtype(dtype)) return CK_ERR_DTYPE;
+    if (tokens == 0) return CK_OK;
+    if (!d_gates || (H > 0 && (!codes || !scales || !grad_out))) return CK_ERR_NULL;
+    if (!ck_aligned_elem(grad_out, dtype) || !ck_aligned_elem(d_gates, dtype)) return CK_ERR_ALIGN;
+    const int64_t grid = ck_ceil_div(tokens, 4);
+    if (grid > 0x7fffffff) return CK_ERR_SHAPE;
+    hipStream_t s = (hipStream_t)stream;
+    const bool vec = aligned8(codes) && ck_aligned16(grad_out) && H % ck::kMxPiece == 0;
+    CK_DISPATCH_DTYPE(dtype, {
+        typedef typename T::storage_t S;
+        if (vec)
+            hipLaunchKernelGGL((ck::combine_bwd_gates_mx8_kernel<T, true>), dim3((unsigned)grid), dim3(256), 0, s,
+                               (const int8_t*)codes, (const uint8_t*)scales, (const S*)grad_out, (S*)d_gates, tokens, (int)k, H);
+        else
+            hipLaunchKernelGGL((ck::combine_bwd_gates_mx8_kernel<T, false>), dim3((unsigned)grid), dim3(256), 0, s,
+                               (const int8_t*)codes, (const uint8_t*)scales, (const S*)grad_out, (S*)d_gates, tokens, (int)k, H);
+    });
+    return ck_launch_status();
+}

@@ -83,6 +83,20 @@ _SIGNATURES = {
     "ck_router_forward": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _i32, _p]),
     "ck_router_weight_grad_workspace_size": (_i64, [_i64, _i64, _i64]),
     "ck_router_weight_grad": (_i32, [_p, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _i32, _p]),
+    "ck_moe_balance_loss_workspace_size": (_i64, [_i64, _i64]),
+    "ck_moe_balance_loss_forward": (
+        _i32,
+        [_p, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i32, _p],
+    ),
+    "ck_moe_balance_loss_backward": (_i32, [_p, _i64, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i32, _p]),
+    "ck_mx8_quantize": (_i32, [_p, _p, _p, _i64, _i64, _i32, _p]),
+    "ck_mx8_dequantize": (_i32, [_p, _p, _p, _i64, _i64, _p, _i64, _i64, _i32, _p]),
+    "ck_swiglu_forward_mx8": (_i32, [_p, _p, _i64, _p, _p, _p, _i64, _p, _p, _i64, _i64, _i64, _i32, _p]),
+    "ck_swiglu_backward_mx8": (_i32, [_p, _p, _i64, _p, _p, _i64, _p, _p, _p, _i64, _p, _i64, _i64, _i32, _p]),
+    "ck_rmsnorm_forward_mx8": (_i32, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _f32, _i32, _p]),
+    "ck_rmsnorm_backward_mx8_workspace_size": (_i64, [_i64, _i64]),
+    "ck_rmsnorm_backward_mx8": (_i32, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i32, _p]),
+    "ck_moe_combine_backward_gates_mx8": (_i32, [_p, _p, _p, _p, _i64, _i64, _i64, _i32, _p]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -846,4 +860,276 @@ def router_topk_softmax_backward(d_weights, weights_f32, selected, d_logits) -> 
             lib.ck_router_topk_softmax_backward(_ptr(d_weights), _ptr(weights_f32), _ptr(selected), _ptr(d_logits),
                                                 d_logits.stride(0), T, E, k, dtype_code(d_logits.dtype), L.stream),
             "ck_router_topk_softmax_backward",
+        )
+
+
+# ---- balance loss ---------------------------------------------------------------------------------------
+def moe_balance_loss_workspace_size(tokens: int, E: int) -> int:
+    return load_library().ck_moe_balance_loss_workspace_size(tokens, E)
+
+
+def _balance_operands(what: str, logits, mask, counts, stats) -> None:
+    T, E = logits.shape
+    if E > 1 and logits.stride(1) != 1:
+        raise ValueError(f"{what}: logits need unit stride over the experts")
+    if mask is not None and (mask.numel() != T or mask.dtype != torch.bool or not mask.is_contiguous()):
+        raise ValueError(f"{what}: the mask is one dense bool per token")
+    for name, t, n in (("counts", counts, E), ("stats", stats, 2)):
+        if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be {n} dense int32")
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.size(0) > 1 else t.size(1)
+
+
+def moe_balance_loss_forward(logits, selected, mask, balance, z, counts, stats, workspace) -> None:
+    """logits [T, E], selected int64 [T, k], mask [T] or None -> balance, z (fp32 scalars), counts [E], stats [2]."""
+    lib = load_library()
+    T, E = logits.shape
+    _balance_operands("moe_balance_loss_forward", logits, mask, counts, stats)
+    if selected.dtype != torch.int64 or selected.dim() != 2 or selected.size(0) != T or not selected.is_contiguous():
+        raise ValueError("moe_balance_loss_forward: selected must be dense int64 [tokens, k]")
+    for t in (balance, z):
+        if t.dtype != torch.float32 or t.numel() != 1:
+            raise ValueError("moe_balance_loss_forward: the losses are one float32 each")
+    with _Launch(logits, selected, mask, balance, z, counts, stats, workspace) as L:
+        _check(
+            lib.ck_moe_balance_loss_forward(
+                _ptr(logits), _row_stride(logits), _ptr(selected), _ptr(mask), _ptr(balance), _ptr(z), _ptr(counts),
+                _ptr(stats), _ptr(workspace), 0 if workspace is None else workspace.numel(), T, E, selected.size(1),
+                dtype_code(logits.dtype), L.stream),
+            "ck_moe_balance_loss_forward",
+        )
+
+
+def moe_balance_loss_backward(logits, mask, counts, stats, balance_grad, z_grad, d_logits, top_k: int) -> None:
+    lib = load_library()
+    T, E = logits.shape
+    _balance_operands("moe_balance_loss_backward", logits, mask, counts, stats)
+    _same_dtype(logits, "moe_balance_loss_backward", d_logits=d_logits)
+    if d_logits.shape != logits.shape or not d_logits.is_contiguous():
+        raise ValueError("moe_balance_loss_backward: d_logits must be dense [tokens, E]")
+    for t in (balance_grad, z_grad):
+        if t is not None and (t.dtype != torch.float32 or t.numel() != 1):
+            raise ValueError("moe_balance_loss_backward: the losses' gradients are one float32 each")
+    with _Launch(logits, mask, counts, stats, balance_grad, z_grad, d_logits) as L:
+        _check(
+            lib.ck_moe_balance_loss_backward(
+                _ptr(logits), _row_stride(logits), _ptr(mask), _ptr(counts), _ptr(stats), _ptr(balance_grad),
+                _ptr(z_grad), _ptr(d_logits), T, E, top_k, dtype_code(logits.dtype), L.stream),
+            "ck_moe_balance_loss_backward",
+        )
+
+
+# ---- activations in 8 bits --------------------------------------------------------------------------------
+MX8_BLOCK = 32
+
+
+def mx8_blocks(H: int) -> int:
+    """Scale bytes of a row of H elements."""
+    return -(-H // MX8_BLOCK)
+
+
+def _mx8_pair(what: str, codes, scales) -> None:
+    """codes int8 [..., H] and scales uint8 [..., ceil(H / 32)], both dense."""
+    if codes.dtype != torch.int8 or scales.dtype != torch.uint8 or codes.dim() < 1:
+        raise ValueError(f"{what}: codes are int8 and scales uint8, got {codes.dtype} and {scales.dtype}")
+    if scales.shape != (*codes.shape[:-1], mx8_blocks(codes.size(-1))):
+        raise ValueError(f"{what}: scales {tuple(scales.shape)} do not go with codes {tuple(codes.shape)}: one per "
+                         f"{MX8_BLOCK} elements of a row")
+    if not codes.is_contiguous() or not scales.is_contiguous():
+        raise ValueError(f"{what}: codes and scales must be contiguous")
+
+
+def _rows_of(t: torch.Tensor) -> tuple[int, int]:
+    H = t.size(-1)
+    return (t.numel() // H if H > 0 else 0), H
+
+
+def mx8_quantize(x, codes, scales) -> None:
+    lib = load_library()
+    _dense("mx8_quantize", x=x)
+    _mx8_pair("mx8_quantize", codes, scales)
+    if codes.numel() != x.numel() or codes.size(-1) != x.size(-1):
+        raise ValueError("mx8_quantize: one code per element")
+    rows, H = _rows_of(x)
+    with _Launch(x, codes, scales) as L:
+        _check(lib.ck_mx8_quantize(_ptr(x), _ptr(codes), _ptr(scales), rows, H, dtype_code(x.dtype), L.stream),
+               "ck_mx8_quantize")
+
+
+def mx8_dequantize(codes, scales, output, index=None, fan: int = 1) -> None:
+    """output = the values of (codes, scales); with `index` (int64 [rows of output]) row r comes from row index[r] // fan."""
+    lib = load_library()
+    _mx8_pair("mx8_dequantize", codes, scales)
+    _dense("mx8_dequantize", output=output, index=index)
+    source_rows, H = _rows_of(codes)
+    rows = _rows_of(output)[0]
+    if output.size(-1) != H or (index is None and rows != source_rows):
+        raise ValueError("mx8_dequantize: the output has the rows' length, and their number unless an index is given")
+    if index is not None and (index.dtype != torch.int64 or index.numel() != rows):
+        raise ValueError("mx8_dequantize: one int64 index per output row")
+    with _Launch(codes, scales, index, output) as L:
+        _check(
+            lib.ck_mx8_dequantize(_ptr(codes), _ptr(scales), _ptr(index), fan, source_rows, _ptr(output), rows, H,
+                                  dtype_code(output.dtype), L.stream),
+            "ck_mx8_dequantize",
+        )
+
+
+def swiglu_forward_mx8(gate, up, output, gate_codes, gate_scales, up_codes, up_scales) -> None:
+    """Two dense tensors of one shape, each with codes and scales of its own."""
+    lib = load_library()
+    _same_dtype(gate, "swiglu_forward_mx8", up=up, output=output)
+    _dense("swiglu_forward_mx8", gate=gate, up=up, output=output)
+    _mx8_pair("swiglu_forward_mx8", gate_codes, gate_scales)
+    _mx8_pair("swiglu_forward_mx8", up_codes, up_scales)
+    if not (gate.shape == up.shape == output.shape == gate_codes.shape == up_codes.shape):
+        raise ValueError("swiglu_forward_mx8: all operands have one shape")
+    rows, H = _rows_of(gate)
+    with _Launch(gate, up, output, gate_codes, gate_scales, up_codes, up_scales) as L:
+        _check(
+            lib.ck_swiglu_forward_mx8(
+                _ptr(gate), _ptr(up), H, _ptr(output), _ptr(gate_codes), _ptr(up_codes), H, _ptr(gate_scales),
+                _ptr(up_scales), mx8_blocks(H), rows, H, dtype_code(gate.dtype), L.stream),
+            "ck_swiglu_forward_mx8",
+        )
+
+
+def swiglu_backward_mx8(gate_codes, gate_scales, up_codes, up_scales, output_grad, gate_grad, up_grad) -> None:
+    lib = load_library()
+    _same_dtype(output_grad, "swiglu_backward_mx8", gate_grad=gate_grad, up_grad=up_grad)
+    _dense("swiglu_backward_mx8", output_grad=output_grad, gate_grad=gate_grad, up_grad=up_grad)
+    _mx8_pair("swiglu_backward_mx8", gate_codes, gate_scales)
+    _mx8_pair("swiglu_backward_mx8", up_codes, up_scales)
+    if not (output_grad.shape == gate_grad.shape == up_grad.shape == gate_codes.shape == up_codes.shape):
+        raise ValueError("swiglu_backward_mx8: all operands have one shape")
+    rows, H = _rows_of(output_grad)
+    with _Launch(gate_codes, gate_scales, up_codes, up_scales, output_grad, gate_grad, up_grad) as L:
+        _check(
+            lib.ck_swiglu_backward_mx8(
+                _ptr(gate_codes), _ptr(up_codes), H, _ptr(gate_scales), _ptr(up_scales), mx8_blocks(H),
+                _ptr(output_grad), _ptr(gate_grad), _ptr(up_grad), H, None, rows, H, dtype_code(output_grad.dtype),
+                L.stream),
+            "ck_swiglu_backward_mx8",
+        )
+
+
+def _halves(t, H: int, size: int):
+    """Addresses of the two halves of a row of 2 H elements: (up, gate)."""
+    first = _ptr(t)
+    return first, None if first is None else first + H * size
+
+
+def swiglu_unchunked_forward_mx8(x, output, codes, scales) -> None:
+    """x [..., 2 H] = (up | gate); codes [..., 2, H] and scales [..., 2, ceil(H / 32)]: each half has blocks of its own."""
+    lib = load_library()
+    _same_dtype(x, "swiglu_unchunked_forward_mx8", output=output)
+    _dense("swiglu_unchunked_forward_mx8", x=x, output=output)
+    _mx8_pair("swiglu_unchunked_forward_mx8", codes, scales)
+    rows, H = _rows_of(output)
+    if x.size(-1) != 2 * H or x.numel() != 2 * output.numel() or codes.numel() != x.numel() or codes.shape[-2:] != (2, H):
+        raise ValueError("swiglu_unchunked_forward_mx8: x [..., 2 H], output [..., H], codes [..., 2, H]")
+    with _Launch(x, output, codes, scales) as L:
+        up, gate = _halves(x, H, x.element_size())
+        up_codes, gate_codes = _halves(codes, H, 1)
+        up_scales, gate_scales = _halves(scales, mx8_blocks(H), 1)
+        _check(
+            lib.ck_swiglu_forward_mx8(gate, up, 2 * H, _ptr(output), gate_codes, up_codes, 2 * H, gate_scales, up_scales,
+                                      2 * mx8_blocks(H), rows, H, dtype_code(x.dtype), L.stream),
+            "ck_swiglu_forward_mx8",
+        )
+
+
+def swiglu_unchunked_backward_mx8(codes, scales, output_grad, x_grad, activation=None) -> None:
+    lib = load_library()
+    _same_dtype(output_grad, "swiglu_unchunked_backward_mx8", x_grad=x_grad, activation=activation)
+    _dense("swiglu_unchunked_backward_mx8", output_grad=output_grad, x_grad=x_grad, activation=activation)
+    _mx8_pair("swiglu_unchunked_backward_mx8", codes, scales)
+    rows, H = _rows_of(output_grad)
+    if x_grad.size(-1) != 2 * H or x_grad.numel() != 2 * output_grad.numel() or codes.numel() != x_grad.numel() or (
+            codes.shape[-2:] != (2, H)) or (activation is not None and activation.shape != output_grad.shape):
+        raise ValueError("swiglu_unchunked_backward_mx8: output_grad [..., H], x_grad [..., 2 H], codes [..., 2, H]")
+    with _Launch(codes, scales, output_grad, x_grad, activation) as L:
+        up_codes, gate_codes = _halves(codes, H, 1)
+        up_scales, gate_scales = _halves(scales, mx8_blocks(H), 1)
+        up_grad, gate_grad = _halves(x_grad, H, x_grad.element_size())
+        _check(
+            lib.ck_swiglu_backward_mx8(gate_codes, up_codes, 2 * H, gate_scales, up_scales, 2 * mx8_blocks(H),
+                                       _ptr(output_grad), gate_grad, up_grad, 2 * H, _ptr(activation), rows, H,
+                                       dtype_code(output_grad.dtype), L.stream),
+            "ck_swiglu_backward_mx8",
+        )
+
+
+def rmsnorm_forward_mx8(x, residual, weight, output, residual_out, codes, scales, rstd, eps: float) -> None:
+    """Rows of x (+ residual, whose sum goes to residual_out) normalised, and kept in 8 bits with their 1 / rms."""
+    lib = load_library()
+    what = "rmsnorm_forward_mx8"
+    _same_dtype(x, what, residual=residual, weight=weight, output=output, residual_out=residual_out)
+    _dense(what, x=x, residual=residual, weight=weight, output=output, residual_out=residual_out, rstd=rstd)
+    _mx8_pair(what, codes, scales)
+    B, H = _rows_of(x)
+    if (residual is None) != (residual_out is None):
+        raise ValueError(f"{what}: residual and residual_out go together")
+    for t in (residual, output, residual_out, codes):
+        if t is not None and t.shape != x.shape:
+            raise ValueError(f"{what}: all operands have the shape of x")
+    if (weight is not None and weight.numel() != H) or rstd.dtype != torch.float32 or rstd.numel() != B:
+        raise ValueError(f"{what}: weight [H], rstd fp32 [rows]")
+    with _Launch(x, residual, weight, output, residual_out, codes, scales, rstd) as L:
+        _check(
+            lib.ck_rmsnorm_forward_mx8(_ptr(x), _ptr(residual), _ptr(weight), _ptr(output), _ptr(residual_out),
+                                       _ptr(codes), _ptr(scales), _ptr(rstd), B, H, eps, dtype_code(x.dtype), L.stream),
+            "ck_rmsnorm_forward_mx8",
+        )
+
+
+def rmsnorm_backward_mx8_workspace_size(B: int, H: int, device: torch.device) -> int:
+    lib = load_library()
+    if device.type != "cuda" or device.index == torch.cuda.current_device():
+        return lib.ck_rmsnorm_backward_mx8_workspace_size(B, H)
+    with torch.cuda.device(device):
+        return lib.ck_rmsnorm_backward_mx8_workspace_size(B, H)
+
+
+def rmsnorm_backward_mx8(codes, scales, weight, output_grad, rstd, sum_grad, x_grad, weight_grad, workspace) -> None:
+    lib = load_library()
+    what = "rmsnorm_backward_mx8"
+    _same_dtype(output_grad, what, weight=weight, sum_grad=sum_grad, x_grad=x_grad, weight_grad=weight_grad)
+    _dense(what, output_grad=output_grad, weight=weight, sum_grad=sum_grad, x_grad=x_grad, weight_grad=weight_grad, rstd=rstd)
+    _mx8_pair(what, codes, scales)
+    B, H = _rows_of(output_grad)
+    for t in (sum_grad, x_grad, codes):
+        if t is not None and t.shape != output_grad.shape:
+            raise ValueError(f"{what}: all operands have the shape of output_grad")
+    if (weight is None) != (weight_grad is None) or (weight is not None and (weight.numel() != H or weight_grad.numel() != H)):
+        raise ValueError(f"{what}: weight and weight_grad go together, [H] each")
+    if rstd.dtype != torch.float32 or rstd.numel() != B:
+        raise ValueError(f"{what}: rstd fp32 [rows]")
+    with _Launch(codes, scales, weight, output_grad, rstd, sum_grad, x_grad, weight_grad, workspace) as L:
+        _check(
+            lib.ck_rmsnorm_backward_mx8(
+                _ptr(codes), _ptr(scales), _ptr(weight), _ptr(output_grad), _ptr(rstd), _ptr(sum_grad), _ptr(x_grad),
+                _ptr(weight_grad), _ptr(workspace), 0 if workspace is None else workspace.numel(), B, H,
+                dtype_code(output_grad.dtype), L.stream),
+            "ck_rmsnorm_backward_mx8",
+        )
+
+
+def moe_combine_backward_gates_mx8(codes, scales, grad_out, d_gates) -> None:
+    """codes [T, k, H] (the expert outputs in 8 bits), grad_out [T, H], d_gates [T, k]; all dense."""
+    lib = load_library()
+    _mx8_pair("moe_combine_backward_gates_mx8", codes, scales)
+    _same_dtype(grad_out, "moe_combine_backward_gates_mx8", d_gates=d_gates)
+    _dense("moe_combine_backward_gates_mx8", grad_out=grad_out, d_gates=d_gates)
+    T, k, H = codes.shape
+    if grad_out.numel() != T * H or d_gates.numel() != T * k:
+        raise ValueError("moe_combine_backward_gates_mx8: codes [T, k, H], grad_out [T, H], d_gates [T, k]")
+    with _Launch(codes, scales, grad_out, d_gates) as L:
+        _check(
+            lib.ck_moe_combine_backward_gates_mx8(_ptr(codes), _ptr(scales), _ptr(grad_out), _ptr(d_gates), T, k, H,
+                                                  dtype_code(grad_out.dtype), L.stream),
+            "ck_moe_combine_backward_gates_mx8",
         )

@@ -25,6 +25,12 @@ from .kernels import (
     embedding_torch,
     fused_residual_add_rmsnorm_cute,
     fused_residual_add_rmsnorm_torch,
+    moe_balance_loss_cute,
+    moe_balance_loss_torch,
+    mx8_dequantize_cute,
+    mx8_dequantize_torch,
+    mx8_quantize_cute,
+    mx8_quantize_torch,
     rmsnorm_cute,
     rmsnorm_torch,
     scattered_experts,

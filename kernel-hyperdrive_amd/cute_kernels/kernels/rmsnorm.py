@@ -19,6 +19,7 @@ from ..cutotune import CutoTuneConfig, CutoTuneParameter, cutotune, get_cartesia
 from ..enums import KernelBackend
 from ..utils import cute_op, ensure_contiguous
 from ._common import check_backend
+from .mx8 import new_mx8
 
 
 def rmsnorm_torch(x: torch.Tensor, weight: torch.Tensor | None, eps: float | None) -> torch.Tensor:
@@ -233,6 +234,110 @@ class _RMSNorm_Cute(torch.autograd.Function):
         return x_grad, weight_grad, None, None, None, None, None, None, None, None
 
 
+@cute_op(
+    f"{LIBRARY_NAME}::rmsnorm_forward_mx8_hip",
+    mutates_args={"output", "residual_output", "codes", "scales", "rmsnorm_denominator"},
+)
+def rmsnorm_forward_mx8_hip(
+    x: torch.Tensor,
+    residual: torch.Tensor | None,
+    weight: torch.Tensor | None,
+    output: torch.Tensor,
+    residual_output: torch.Tensor | None,
+    codes: torch.Tensor,
+    scales: torch.Tensor,
+    rmsnorm_denominator: torch.Tensor,
+    eps: float,
+) -> None:
+    _C.rmsnorm_forward_mx8(x, residual, weight, output, residual_output, codes, scales, rmsnorm_denominator, eps)
+
+
+@cute_op(f"{LIBRARY_NAME}::rmsnorm_backward_mx8_hip", mutates_args={"x_grad", "weight_grad"})
+def rmsnorm_backward_mx8_hip(
+    codes: torch.Tensor,
+    scales: torch.Tensor,
+    weight: torch.Tensor | None,
+    output_grad: torch.Tensor,
+    rmsnorm_denominator: torch.Tensor,
+    sum_grad: torch.Tensor | None,
+    x_grad: torch.Tensor,
+    weight_grad: torch.Tensor | None,
+) -> None:
+    workspace = None
+    if weight is not None:
+        hidden_size = output_grad.size(-1)
+        num_rows = output_grad.numel() // hidden_size if hidden_size > 0 else 0
+        nbytes = _C.rmsnorm_backward_mx8_workspace_size(num_rows, hidden_size, output_grad.device)
+        workspace = torch.empty(max(nbytes, 16), device=output_grad.device, dtype=torch.uint8)
+    _C.rmsnorm_backward_mx8(
+        codes, scales, weight, output_grad, rmsnorm_denominator, sum_grad, x_grad, weight_grad, workspace
+    )
+
+
+def _check_mx8_arguments(x: torch.Tensor, weight: torch.Tensor | None, memory_efficient: bool) -> None:
+    if weight is not None:
+        assert weight.dim() == 1, "weight should be 1D"
+        assert weight.size(-1) == x.size(-1), "hidden size for x and weight tensor is different"
+        assert weight.type() == x.type(), "tensors weight and y should have same dtype"
+    if memory_efficient:
+        # 1 / rms is that of the exact row: it cannot be had again from the kept one
+        raise ValueError("checkpoint_8bit saves 1 / rms and does not go with memory_efficient")
+    _check_row_length(x.size(-1))
+
+
+class _RMSNormMX8_Cute(torch.autograd.Function):
+    """As ``_RMSNorm_Cute``, with x saved in 8 bits (see mx8.py) by the forward's own pass; 1 / rms is saved as well."""
+
+    @staticmethod
+    @ensure_contiguous
+    def forward(ctx, x: torch.Tensor, weight: torch.Tensor | None, eps: float | None) -> torch.Tensor:
+        if eps is None:
+            eps = torch.finfo(x.dtype).eps
+        ctx.shape = x.shape
+        rows = x.shape if x.dim() > 1 else (1, x.numel())
+        hidden_size = x.size(-1)
+        num_rows = x.numel() // hidden_size if hidden_size > 0 else 0
+        output = torch.empty_like(x)
+        codes, scales = new_mx8(rows, x.device)
+        rmsnorm_denominator = torch.empty(num_rows, device=x.device, dtype=torch.float32)
+        rmsnorm_forward_mx8_hip(
+            x=x.view(rows),
+            residual=None,
+            weight=weight,
+            output=output.view(rows),
+            residual_output=None,
+            codes=codes,
+            scales=scales,
+            rmsnorm_denominator=rmsnorm_denominator,
+            eps=eps,
+        )
+        ctx.save_for_backward(codes, scales, weight, rmsnorm_denominator)
+        return output
+
+    @staticmethod
+    @ensure_contiguous
+    def backward(ctx, output_grad: torch.Tensor):
+        codes, scales, weight, rmsnorm_denominator = ctx.saved_tensors
+        output_grad = output_grad.view(codes.shape)
+        x_grad = torch.empty_like(output_grad)
+        weight_grad = None if weight is None else torch.empty_like(weight)
+        rmsnorm_backward_mx8_hip(
+            codes=codes,
+            scales=scales,
+            weight=weight,
+            output_grad=output_grad,
+            rmsnorm_denominator=rmsnorm_denominator,
+            sum_grad=None,
+            x_grad=x_grad,
+            weight_grad=weight_grad,
+        )
+        return x_grad.view(ctx.shape), weight_grad, None
+
+
+def _wants_grad(*tensors: torch.Tensor | None) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 def rmsnorm_cute(
     x: torch.Tensor,
     weight: torch.Tensor | None,
@@ -244,7 +349,14 @@ def rmsnorm_cute(
     BLOCK_SIZE_B_backward: int = CutoTuneParameter(),
     BLOCK_SIZE_H_forward: int = CutoTuneParameter(),
     BLOCK_SIZE_H_backward: int = CutoTuneParameter(),
+    checkpoint_8bit: bool = False,
 ) -> torch.Tensor:
+    """``checkpoint_8bit``: keep x for the backward in 8 bits (see mx8.py); the output is that of the exact rows, the gradients
+    are those at the kept rows with the exact rows' 1 / rms.  Not with ``memory_efficient``; the tunables have no meaning there."""
+    if checkpoint_8bit:
+        _check_mx8_arguments(x, weight, memory_efficient)
+        if _wants_grad(x, weight):
+            return _RMSNormMX8_Cute.apply(x, weight, eps)
     return _RMSNorm_Cute.apply(
         x,
         weight,

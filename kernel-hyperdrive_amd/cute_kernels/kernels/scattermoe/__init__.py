@@ -1,3 +1,4 @@
+from .balance import moe_balance_loss_cute, moe_balance_loss_torch
 from .moe_hip import Experts_HIP, Experts_Triton, MoE_HIP, MoE_Triton, moe_router, moe_sort, router_topk_softmax
 from .moe_torch import Experts_Torch, MoE_Torch
 from .ops import (

@@ -12,6 +12,7 @@ from ... import _C
 from ...constants import LIBRARY_NAME
 from ...utils import cute_op
 from ..swiglu_unchunked import swiglu_unchunked_cute, swiglu_unchunked_torch
+from .balance import moe_balance_loss_cute
 from .moe_torch import Experts_Torch, MoE_Torch
 from .ops import scattered_experts, scattered_glu_experts
 
@@ -276,6 +277,19 @@ class MoE_HIP(MoE_Torch):
     # GEMM's are, but summed in another order: a few differ in the last bit, which can turn a near-tie the other way.
     # False keeps ``self.gate`` as a module call.
     fuse_router_linear = True
+    # Save what the experts' backward needs in 8 bits (see kernels/mx8.py): at 8192 tokens of 4096, 8 experts of 14336 and
+    # top-2 0.59 instead of 1.61 GB per call.  Outputs stay the same, gradients are those at the kept values.  Needs a
+    # SwiGLU between the expert products and no expert bias.
+    checkpoint_8bit = False
+
+    def balance_loss(
+        self, router_logits: torch.Tensor, token_mask: torch.Tensor | None = None
+    ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """``moe_balance_loss_cute`` of the logits this layer's forward returned, with the experts it selected by them;
+        ``token_mask``: one bool per token, in any shape."""
+        if token_mask is not None:
+            token_mask = token_mask.reshape(-1)
+        return moe_balance_loss_cute(router_logits, None, token_mask, top_k=self.top_k)
 
     def _compute_routing_weights(self, hidden_states: torch.Tensor):
         if not (
@@ -304,7 +318,10 @@ class MoE_HIP(MoE_Torch):
             and self.intermediate_size % 128 == 0
             and self.hidden_size % 8 == 0
         )
-        if self.fuse_swiglu and fusable and self.act in (swiglu_unchunked_cute, swiglu_unchunked_torch):
+        is_swiglu = self.act in (swiglu_unchunked_cute, swiglu_unchunked_torch)
+        if self.checkpoint_8bit and not (is_swiglu and self.c_fc.bias is None and self.c_proj.bias is None):
+            raise ValueError("checkpoint_8bit needs swiglu_unchunked between the expert products and no expert bias")
+        if self.checkpoint_8bit or (self.fuse_swiglu and fusable and is_swiglu):
             return scattered_glu_experts(
                 hidden_states,
                 self.c_fc.weight.permute(0, 2, 1),
@@ -314,6 +331,7 @@ class MoE_HIP(MoE_Torch):
                 sorted_scattered_idxs,
                 expert_offsets,
                 router_weights,
+                self.checkpoint_8bit,
             )
 
         # [T, H] -> rows gathered per expert -> [T * k, I or 2I], grouped by expert

@@ -31,6 +31,8 @@ from ... import _C
 from ...constants import LIBRARY_NAME
 from ...cutotune import CutoTuneConfig, CutoTuneParameter, cutotune, get_cartesian_product_cutotune_configs
 from ...utils import cute_op
+from ..mx8 import mx8_dequantize_hip, mx8_quantize_hip, new_mx8
+from ..swiglu_unchunked import swiglu_unchunked_backward_mx8_hip
 
 
 torch._dynamo.config.capture_scalar_outputs = True
@@ -259,6 +261,14 @@ def _sum_over_slots(d_expanded_input: torch.Tensor, tokens: int, k: int) -> torc
 def moe_combine_backward_gates(expanded: torch.Tensor, grad_out: torch.Tensor, d_gates: torch.Tensor) -> None:
     """d_gates[t, j] = <expanded[t, j], grad_out[t]>  (the reference's bmm(expanded[T,k,H], grad_out[T,H,1]))."""
     _C.moe_combine_backward_gates(expanded.contiguous(), grad_out.contiguous(), d_gates)
+
+
+@cute_op(f"{LIBRARY_NAME}::moe_combine_backward_gates_mx8", mutates_args={"d_gates"})
+def moe_combine_backward_gates_mx8(
+    codes: torch.Tensor, scales: torch.Tensor, grad_out: torch.Tensor, d_gates: torch.Tensor
+) -> None:
+    """As ``moe_combine_backward_gates``, with the expert outputs in 8 bits."""
+    _C.moe_combine_backward_gates_mx8(codes, scales, grad_out.contiguous(), d_gates)
 
 
 @cute_op(f"{LIBRARY_NAME}::expert_bias_forward", mutates_args={"y"})
@@ -505,7 +515,132 @@ class _ScatteredGLUExperts(torch.autograd.Function):
         return d_input, d_w_fc, d_w_proj, None, None, None, None, d_gates
 
 
-def scattered_glu_experts(inputs, w_fc, w_proj, k, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates):
+class _ScatteredGLUExpertsMX8(torch.autograd.Function):
+    """``_ScatteredGLUExperts`` with what its backward needs - x, c_fc's output and the expert outputs - saved in 8 bits
+    (see mx8.py), and the activation not saved at all but recomputed by the pass that computes h's gradient.  The output
+    does not change; the gradients are those at the kept values."""
+
+    @staticmethod
+    def forward(ctx, x, w_fc, w_proj, k, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates):
+        num_slots = sorted_expert_idxs.size(0)
+        half = w_proj.size(1)
+        x = x.contiguous()
+        h = torch.empty(num_slots, 2 * half, device=x.device, dtype=x.dtype)
+        act = torch.empty(num_slots, half, device=x.device, dtype=x.dtype)
+        scatter2scatter_glu(
+            X=x,
+            W=w_fc,
+            sorted_scattered_idxs=sorted_scattered_idxs,
+            expert_offsets=expert_offsets,
+            h=h,
+            act=act,
+            FAN_OUT=k,
+            x_grouped=False,
+        )
+        h_codes, h_scales = new_mx8((num_slots, 2, half), x.device)
+        mx8_quantize_hip(h.view(num_slots, 2, half), h_codes, h_scales)
+        del h
+        expanded = torch.empty(num_slots, w_proj.size(-1), device=x.device, dtype=x.dtype)
+        scatter2scatter(
+            X=act,
+            W=w_proj,
+            sorted_expert_idxs=sorted_expert_idxs,
+            sorted_scattered_idxs=sorted_scattered_idxs,
+            out=expanded,
+            FAN_OUT=1,
+            x_grouped=True,
+            y_grouped=False,
+            expert_offsets=expert_offsets,
+        )
+        del act
+        expanded = expanded.view(gates.size(0), gates.size(1), expanded.size(-1))
+        output = torch.empty(gates.size(0), expanded.size(-1), device=x.device, dtype=x.dtype)
+        moe_combine_forward(expanded=expanded, gates=gates, out=output)
+        y_codes, y_scales = new_mx8(expanded.shape, x.device)
+        mx8_quantize_hip(expanded, y_codes, y_scales)
+        x_codes, x_scales = new_mx8(x.shape, x.device)
+        mx8_quantize_hip(x, x_codes, x_scales)
+        ctx.save_for_backward(
+            w_fc, w_proj, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates, x_codes, x_scales, h_codes,
+            h_scales, y_codes, y_scales
+        )
+        ctx.k = k
+        return output
+
+    @staticmethod
+    def backward(ctx, grad_out):
+        (w_fc, w_proj, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates, x_codes, x_scales, h_codes,
+         h_scales, y_codes, y_scales) = ctx.saved_tensors
+        k = ctx.k
+        E = w_fc.size(0)
+        num_slots, half = sorted_expert_idxs.size(0), w_proj.size(1)
+        device, dtype = grad_out.device, grad_out.dtype
+        grad_out = grad_out.contiguous()
+
+        d_gates = torch.empty_like(gates)
+        moe_combine_backward_gates_mx8(y_codes, y_scales, grad_out, d_gates)
+        # grad_out rows times their routing weight, in expert-grouped order
+        grouped_grad_out = torch.empty(num_slots, grad_out.size(1), device=device, dtype=dtype)
+        group(
+            A=grad_out,
+            sorted_expert_idxs=sorted_scattered_idxs,
+            out=grouped_grad_out,
+            coeff=gates.flatten(),
+            fan_out=gates.size(1),
+        )
+
+        d_act = torch.empty(num_slots, half, device=device, dtype=dtype)
+        scatter2scatter(
+            X=grouped_grad_out,
+            W=w_proj.permute(0, 2, 1),
+            sorted_expert_idxs=sorted_expert_idxs,
+            sorted_scattered_idxs=sorted_scattered_idxs,
+            out=d_act,
+            FAN_OUT=1,
+            x_grouped=True,
+            y_grouped=True,
+            expert_offsets=expert_offsets,
+        )
+        # one pass over the kept h gives its gradient and, again, the activation
+        d_h = torch.empty(num_slots, 2 * half, device=device, dtype=dtype)
+        act = torch.empty(num_slots, half, device=device, dtype=dtype)
+        swiglu_unchunked_backward_mx8_hip(
+            codes=h_codes, scales=h_scales, output_grad=d_act, x_grad=d_h, activation=act
+        )
+        del d_act
+        d_w_proj = torch.empty_like(w_proj)
+        group_bwd_W(DY=grouped_grad_out, X=act, expert_offsets=expert_offsets, DW=d_w_proj, E=E)
+        del act, grouped_grad_out
+
+        grouped_x = torch.empty(num_slots, x_codes.size(1), dtype=dtype, device=device)
+        mx8_dequantize_hip(x_codes, x_scales, grouped_x, sorted_scattered_idxs, k)
+        d_w_fc = torch.empty_like(w_fc)
+        group_bwd_W(DY=d_h, X=grouped_x, expert_offsets=expert_offsets, DW=d_w_fc, E=E)
+        d_expanded_input = grouped_x  # reused once the weight gradient has consumed it
+        scatter2scatter(
+            X=d_h,
+            W=w_fc.permute(0, 2, 1),
+            sorted_expert_idxs=sorted_expert_idxs,
+            sorted_scattered_idxs=sorted_scattered_idxs,
+            out=d_expanded_input,
+            FAN_OUT=1,
+            x_grouped=True,
+            y_grouped=False,
+            expert_offsets=expert_offsets,
+        )
+        d_input = _sum_over_slots(d_expanded_input, x_codes.size(0), k)
+        # x, w_fc, w_proj, k, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates
+        return d_input, d_w_fc, d_w_proj, None, None, None, None, d_gates
+
+
+def scattered_glu_experts(
+    inputs, w_fc, w_proj, k, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates, checkpoint_8bit=False
+):
+    """``checkpoint_8bit``: keep what the backward needs in 8 bits (``_ScatteredGLUExpertsMX8``)."""
+    if checkpoint_8bit and torch.is_grad_enabled() and any(t.requires_grad for t in (inputs, w_fc, w_proj, gates)):
+        return _ScatteredGLUExpertsMX8.apply(
+            inputs, w_fc, w_proj, k, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates
+        )
     return _ScatteredGLUExperts.apply(
         inputs, w_fc, w_proj, k, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates
     )

@@ -15,6 +15,7 @@ from ..enums import KernelBackend
 from ..math import divide_if_divisible
 from ..utils import cute_op, ensure_contiguous
 from ._common import check_backend, workgroup_size
+from .mx8 import new_mx8
 
 
 def swiglu_unchunked_torch(x: torch.Tensor) -> torch.Tensor:
@@ -96,6 +97,48 @@ class _SwigluUnchunked_Cute(torch.autograd.Function):
         return x_grad, None, None, None, None, None, None
 
 
+@cute_op(f"{LIBRARY_NAME}::swiglu_unchunked_forward_mx8_hip", mutates_args={"output", "codes", "scales"})
+def swiglu_unchunked_forward_mx8_hip(
+    x: torch.Tensor, output: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor
+) -> None:
+    _C.swiglu_unchunked_forward_mx8(x, output, codes, scales)
+
+
+@cute_op(f"{LIBRARY_NAME}::swiglu_unchunked_backward_mx8_hip", mutates_args={"x_grad", "activation"})
+def swiglu_unchunked_backward_mx8_hip(
+    codes: torch.Tensor,
+    scales: torch.Tensor,
+    output_grad: torch.Tensor,
+    x_grad: torch.Tensor,
+    activation: torch.Tensor | None = None,
+) -> None:
+    """``activation``: also written, with the forward's output at the kept inputs."""
+    _C.swiglu_unchunked_backward_mx8(codes, scales, output_grad, x_grad, activation)
+
+
+class _SwigluUnchunkedMX8_Cute(torch.autograd.Function):
+    """As ``_SwigluUnchunked_Cute``, with x saved in 8 bits (see mx8.py; each half of a row has blocks of its own)."""
+
+    @staticmethod
+    @ensure_contiguous
+    def forward(ctx, x: torch.Tensor) -> torch.Tensor:
+        h = divide_if_divisible(x.size(-1), 2, "last dimension of x must be even")
+        output = torch.empty(*x.size()[:-1], h, device=x.device, dtype=x.dtype)
+        codes, scales = new_mx8((*x.size()[:-1], 2, h), x.device)
+        swiglu_unchunked_forward_mx8_hip(x=x, output=output, codes=codes, scales=scales)
+        ctx.save_for_backward(codes, scales)
+        return output
+
+    @staticmethod
+    @ensure_contiguous
+    def backward(ctx, output_grad: torch.Tensor):
+        codes, scales = ctx.saved_tensors
+        h = output_grad.size(-1)
+        x_grad = torch.empty(*output_grad.size()[:-1], 2 * h, device=output_grad.device, dtype=output_grad.dtype)
+        swiglu_unchunked_backward_mx8_hip(codes=codes, scales=scales, output_grad=output_grad, x_grad=x_grad)
+        return x_grad
+
+
 def swiglu_unchunked_cute(
     x: torch.Tensor,
     kernel_backend_forward: KernelBackend = CutoTuneParameter(),
@@ -104,7 +147,12 @@ def swiglu_unchunked_cute(
     BLOCK_SIZE_H_forward: int = CutoTuneParameter(),
     BLOCK_SIZE_B_backward: int = CutoTuneParameter(),
     BLOCK_SIZE_H_backward: int = CutoTuneParameter(),
+    checkpoint_8bit: bool = False,
 ) -> torch.Tensor:
+    """``checkpoint_8bit``: keep x for the backward in 8 bits (see mx8.py); the output is that of the exact x, the gradient
+    that at the kept values.  The other tunables have no meaning there."""
+    if checkpoint_8bit and torch.is_grad_enabled() and x.requires_grad:
+        return _SwigluUnchunkedMX8_Cute.apply(x)
     return _SwigluUnchunked_Cute.apply(
         x,
         kernel_backend_forward,

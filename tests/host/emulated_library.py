@@ -102,8 +102,8 @@ class _GuardedCall:
         else:
             copy = fence - nbytes
             copy -= (copy - lo) % 16
-        if t.dtype == torch.uint8:
-            # a workspace: its contents are undefined by contract, so a kernel that reads a byte of it before writing
+        if t.dtype == torch.uint8 and t.dim() == 1:
+            # a workspace (scale bytes are matrices): its contents are undefined by contract, so a kernel that reads a byte of it before writing
             # it reads ones here (NaNs as floats, -1 as integers) and the results show it
             ctypes.memset(copy, 0xFF, nbytes)
         else:

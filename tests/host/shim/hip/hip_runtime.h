@@ -312,6 +312,12 @@ inline int emu_readfirstlane(int v) {
     return emu::wave_instruction(v, [](auto lane) { return lane(0); });
 }
 #define __builtin_amdgcn_readfirstlane(v) emu_readfirstlane(v)
+// v_mov_b32 with a quad_perm control (the only DPP form the kernels use): lane l reads lane 4 (l / 4) + (ctrl >> 2 (l % 4)) % 4
+inline int emu_quad_perm(int v, int ctrl) {
+    const int me = __lane_id();
+    return emu::wave_instruction(v, [me, ctrl](auto lane) { return lane(me / 4 * 4 + ((ctrl >> (2 * (me % 4))) & 3)); });
+}
+#define __builtin_amdgcn_mov_dpp(v, ctrl, row_mask, bank_mask, bound_ctrl) emu_quad_perm(v, ctrl)
 #define __builtin_amdgcn_s_barrier() emu::sync(emu::g_block)
 // The lanes of a wavefront run in lock-step on the hardware; here they run freely between the instructions that make
 // them meet.  Where a kernel lets lanes of one wave talk through memory and relies on the lock-step, it says so with a
