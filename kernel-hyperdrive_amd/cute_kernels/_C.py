@@ -161,17 +161,28 @@ def _require_gpu(*tensors: torch.Tensor | None) -> torch.device:
 class _Launch:
     """Context for one native call: the tensors' device made current, its stream fetched."""
 
-    __slots__ = ("device", "guard", "stream")
+    __slots__ = ("index", "guard", "stream")
 
     def __init__(self, *tensors):
-        self.device = _require_gpu(*tensors)
+        # one device number per tensor (-1: not on a GPU); anything else is looked at, and refused, by _require_gpu
+        index = -1
+        for t in tensors:
+            if t is not None:
+                i = t.get_device()
+                if i != index:
+                    if index >= 0 or i < 0:
+                        _require_gpu(*tensors)
+                    index = i
+        if index < 0:
+            _require_gpu(*tensors)
+        self.index = index
         self.guard = None
 
     def __enter__(self):
-        if self.device.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(self.device)
+        if self.index != torch._C._cuda_getDevice():
+            self.guard = torch.cuda.device(self.index)
             self.guard.__enter__()
-        self.stream = torch.cuda.current_stream().cuda_stream
+        self.stream = torch._C._cuda_getCurrentRawStream(self.index)
         return self
 
     def __exit__(self, *exc):
@@ -868,36 +879,33 @@ def moe_balance_loss_workspace_size(tokens: int, E: int) -> int:
     return load_library().ck_moe_balance_loss_workspace_size(tokens, E)
 
 
-def _balance_operands(what: str, logits, mask, counts, stats) -> None:
+def _balance_operands(what: str, logits, mask, counts, stats) -> tuple[int, int, int]:
+    """(tokens, experts, distance of the logits' rows)"""
     T, E = logits.shape
-    if E > 1 and logits.stride(1) != 1:
+    row, column = logits.stride()
+    if column != 1 and E > 1:
         raise ValueError(f"{what}: logits need unit stride over the experts")
     if mask is not None and (mask.numel() != T or mask.dtype != torch.bool or not mask.is_contiguous()):
         raise ValueError(f"{what}: the mask is one dense bool per token")
-    for name, t, n in (("counts", counts, E), ("stats", stats, 2)):
+    for t, n in ((counts, E), (stats, 2)):
         if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
-            raise ValueError(f"{what}: {name} must be {n} dense int32")
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.size(0) > 1 else t.size(1)
+            raise ValueError(f"{what}: counts are dense int32 [experts], stats dense int32 [2]")
+    return T, E, row if T > 1 else E
 
 
 def moe_balance_loss_forward(logits, selected, mask, balance, z, counts, stats, workspace) -> None:
     """logits [T, E], selected int64 [T, k], mask [T] or None -> balance, z (fp32 scalars), counts [E], stats [2]."""
     lib = load_library()
-    T, E = logits.shape
-    _balance_operands("moe_balance_loss_forward", logits, mask, counts, stats)
+    T, E, row = _balance_operands("moe_balance_loss_forward", logits, mask, counts, stats)
     if selected.dtype != torch.int64 or selected.dim() != 2 or selected.size(0) != T or not selected.is_contiguous():
         raise ValueError("moe_balance_loss_forward: selected must be dense int64 [tokens, k]")
-    for t in (balance, z):
-        if t.dtype != torch.float32 or t.numel() != 1:
-            raise ValueError("moe_balance_loss_forward: the losses are one float32 each")
+    if balance.dtype != torch.float32 or z.dtype != torch.float32 or balance.numel() != 1 or z.numel() != 1:
+        raise ValueError("moe_balance_loss_forward: the losses are one float32 each")
     with _Launch(logits, selected, mask, balance, z, counts, stats, workspace) as L:
         _check(
             lib.ck_moe_balance_loss_forward(
-                _ptr(logits), _row_stride(logits), _ptr(selected), _ptr(mask), _ptr(balance), _ptr(z), _ptr(counts),
-                _ptr(stats), _ptr(workspace), 0 if workspace is None else workspace.numel(), T, E, selected.size(1),
+                _ptr(logits), row, _ptr(selected), _ptr(mask), _ptr(balance), _ptr(z), _ptr(counts), _ptr(stats),
+                _ptr(workspace), 0 if workspace is None else workspace.numel(), T, E, selected.size(1),
                 dtype_code(logits.dtype), L.stream),
             "ck_moe_balance_loss_forward",
         )
@@ -905,19 +913,17 @@ def moe_balance_loss_forward(logits, selected, mask, balance, z, counts, stats, 
 
 def moe_balance_loss_backward(logits, mask, counts, stats, balance_grad, z_grad, d_logits, top_k: int) -> None:
     lib = load_library()
-    T, E = logits.shape
-    _balance_operands("moe_balance_loss_backward", logits, mask, counts, stats)
-    _same_dtype(logits, "moe_balance_loss_backward", d_logits=d_logits)
-    if d_logits.shape != logits.shape or not d_logits.is_contiguous():
-        raise ValueError("moe_balance_loss_backward: d_logits must be dense [tokens, E]")
+    T, E, row = _balance_operands("moe_balance_loss_backward", logits, mask, counts, stats)
+    if d_logits.dtype != logits.dtype or d_logits.shape != logits.shape or not d_logits.is_contiguous():
+        raise ValueError("moe_balance_loss_backward: d_logits must be dense [tokens, experts] of the logits' dtype")
     for t in (balance_grad, z_grad):
         if t is not None and (t.dtype != torch.float32 or t.numel() != 1):
             raise ValueError("moe_balance_loss_backward: the losses' gradients are one float32 each")
     with _Launch(logits, mask, counts, stats, balance_grad, z_grad, d_logits) as L:
         _check(
             lib.ck_moe_balance_loss_backward(
-                _ptr(logits), _row_stride(logits), _ptr(mask), _ptr(counts), _ptr(stats), _ptr(balance_grad),
-                _ptr(z_grad), _ptr(d_logits), T, E, top_k, dtype_code(logits.dtype), L.stream),
+                _ptr(logits), row, _ptr(mask), _ptr(counts), _ptr(stats), _ptr(balance_grad), _ptr(z_grad),
+                _ptr(d_logits), T, E, top_k, dtype_code(logits.dtype), L.stream),
             "ck_moe_balance_loss_backward",
         )
 
@@ -933,27 +939,35 @@ def mx8_blocks(H: int) -> int:
 
 def _mx8_pair(what: str, codes, scales) -> None:
     """codes int8 [..., H] and scales uint8 [..., ceil(H / 32)], both dense."""
-    if codes.dtype != torch.int8 or scales.dtype != torch.uint8 or codes.dim() < 1:
+    if codes.dtype != torch.int8 or scales.dtype != torch.uint8:
         raise ValueError(f"{what}: codes are int8 and scales uint8, got {codes.dtype} and {scales.dtype}")
-    if scales.shape != (*codes.shape[:-1], mx8_blocks(codes.size(-1))):
-        raise ValueError(f"{what}: scales {tuple(scales.shape)} do not go with codes {tuple(codes.shape)}: one per "
+    shape = codes.shape
+    if scales.shape != (*shape[:-1], -(-shape[-1] // MX8_BLOCK)):
+        raise ValueError(f"{what}: scales {tuple(scales.shape)} do not go with codes {tuple(shape)}: one per "
                          f"{MX8_BLOCK} elements of a row")
     if not codes.is_contiguous() or not scales.is_contiguous():
         raise ValueError(f"{what}: codes and scales must be contiguous")
 
 
-def _rows_of(t: torch.Tensor) -> tuple[int, int]:
-    H = t.size(-1)
-    return (t.numel() // H if H > 0 else 0), H
+def _rows_alike(what: str, first, *others) -> tuple[int, int]:
+    """(rows, row length) of tensors that are dense and of one shape and dtype."""
+    shape, dtype = first.shape, first.dtype
+    if not first.is_contiguous():
+        raise ValueError(f"{what}: operands must be contiguous")
+    for t in others:
+        if t is not None and (t.dtype != dtype or t.shape != shape or not t.is_contiguous()):
+            raise ValueError(f"{what}: operands must be contiguous and of one shape and dtype: {tuple(t.shape)} {t.dtype}, "
+                             f"the first {tuple(shape)} {dtype}")
+    H = shape[-1]
+    return (first.numel() // H if H > 0 else 0), H
 
 
 def mx8_quantize(x, codes, scales) -> None:
     lib = load_library()
-    _dense("mx8_quantize", x=x)
+    rows, H = _rows_alike("mx8_quantize", x)
     _mx8_pair("mx8_quantize", codes, scales)
-    if codes.numel() != x.numel() or codes.size(-1) != x.size(-1):
+    if codes.shape != x.shape:
         raise ValueError("mx8_quantize: one code per element")
-    rows, H = _rows_of(x)
     with _Launch(x, codes, scales) as L:
         _check(lib.ck_mx8_quantize(_ptr(x), _ptr(codes), _ptr(scales), rows, H, dtype_code(x.dtype), L.stream),
                "ck_mx8_quantize")
@@ -963,12 +977,11 @@ def mx8_dequantize(codes, scales, output, index=None, fan: int = 1) -> None:
     """output = the values of (codes, scales); with `index` (int64 [rows of output]) row r comes from row index[r] // fan."""
     lib = load_library()
     _mx8_pair("mx8_dequantize", codes, scales)
-    _dense("mx8_dequantize", output=output, index=index)
-    source_rows, H = _rows_of(codes)
-    rows = _rows_of(output)[0]
-    if output.size(-1) != H or (index is None and rows != source_rows):
+    rows, H = _rows_alike("mx8_dequantize", output)
+    source_rows = codes.numel() // H if H > 0 else 0
+    if codes.shape[-1] != H or (index is None and rows != source_rows):
         raise ValueError("mx8_dequantize: the output has the rows' length, and their number unless an index is given")
-    if index is not None and (index.dtype != torch.int64 or index.numel() != rows):
+    if index is not None and (index.dtype != torch.int64 or index.numel() != rows or not index.is_contiguous()):
         raise ValueError("mx8_dequantize: one int64 index per output row")
     with _Launch(codes, scales, index, output) as L:
         _check(
@@ -978,106 +991,97 @@ def mx8_dequantize(codes, scales, output, index=None, fan: int = 1) -> None:
         )
 
 
-def swiglu_forward_mx8(gate, up, output, gate_codes, gate_scales, up_codes, up_scales) -> None:
-    """Two dense tensors of one shape, each with codes and scales of its own."""
+def swiglu_forward_mx8(gate, up, output, codes, scales) -> None:
+    """Two dense tensors of one shape; codes [2, ...] and scales: gate's, then up's."""
     lib = load_library()
-    _same_dtype(gate, "swiglu_forward_mx8", up=up, output=output)
-    _dense("swiglu_forward_mx8", gate=gate, up=up, output=output)
-    _mx8_pair("swiglu_forward_mx8", gate_codes, gate_scales)
-    _mx8_pair("swiglu_forward_mx8", up_codes, up_scales)
-    if not (gate.shape == up.shape == output.shape == gate_codes.shape == up_codes.shape):
-        raise ValueError("swiglu_forward_mx8: all operands have one shape")
-    rows, H = _rows_of(gate)
-    with _Launch(gate, up, output, gate_codes, gate_scales, up_codes, up_scales) as L:
+    rows, H = _rows_alike("swiglu_forward_mx8", gate, up, output)
+    _mx8_pair("swiglu_forward_mx8", codes, scales)
+    if codes.shape != (2, *gate.shape):
+        raise ValueError("swiglu_forward_mx8: codes [2, ...] of the operands' shape")
+    with _Launch(gate, up, output, codes, scales) as L:
+        c, s, blocks = _ptr(codes), _ptr(scales), mx8_blocks(H)
+        n = rows * H
         _check(
-            lib.ck_swiglu_forward_mx8(
-                _ptr(gate), _ptr(up), H, _ptr(output), _ptr(gate_codes), _ptr(up_codes), H, _ptr(gate_scales),
-                _ptr(up_scales), mx8_blocks(H), rows, H, dtype_code(gate.dtype), L.stream),
+            lib.ck_swiglu_forward_mx8(_ptr(gate), _ptr(up), H, _ptr(output), c, c + n if n else c, H, s,
+                                      s + rows * blocks if n else s, blocks, rows, H, dtype_code(gate.dtype), L.stream),
             "ck_swiglu_forward_mx8",
         )
 
 
-def swiglu_backward_mx8(gate_codes, gate_scales, up_codes, up_scales, output_grad, gate_grad, up_grad) -> None:
+def swiglu_backward_mx8(codes, scales, output_grad, gate_grad, up_grad) -> None:
     lib = load_library()
-    _same_dtype(output_grad, "swiglu_backward_mx8", gate_grad=gate_grad, up_grad=up_grad)
-    _dense("swiglu_backward_mx8", output_grad=output_grad, gate_grad=gate_grad, up_grad=up_grad)
-    _mx8_pair("swiglu_backward_mx8", gate_codes, gate_scales)
-    _mx8_pair("swiglu_backward_mx8", up_codes, up_scales)
-    if not (output_grad.shape == gate_grad.shape == up_grad.shape == gate_codes.shape == up_codes.shape):
-        raise ValueError("swiglu_backward_mx8: all operands have one shape")
-    rows, H = _rows_of(output_grad)
-    with _Launch(gate_codes, gate_scales, up_codes, up_scales, output_grad, gate_grad, up_grad) as L:
+    rows, H = _rows_alike("swiglu_backward_mx8", output_grad, gate_grad, up_grad)
+    _mx8_pair("swiglu_backward_mx8", codes, scales)
+    if codes.shape != (2, *output_grad.shape):
+        raise ValueError("swiglu_backward_mx8: codes [2, ...] of the operands' shape")
+    with _Launch(codes, scales, output_grad, gate_grad, up_grad) as L:
+        c, s, blocks = _ptr(codes), _ptr(scales), mx8_blocks(H)
+        n = rows * H
         _check(
-            lib.ck_swiglu_backward_mx8(
-                _ptr(gate_codes), _ptr(up_codes), H, _ptr(gate_scales), _ptr(up_scales), mx8_blocks(H),
-                _ptr(output_grad), _ptr(gate_grad), _ptr(up_grad), H, None, rows, H, dtype_code(output_grad.dtype),
-                L.stream),
+            lib.ck_swiglu_backward_mx8(c, c + n if n else c, H, s, s + rows * blocks if n else s, blocks,
+                                       _ptr(output_grad), _ptr(gate_grad), _ptr(up_grad), H, None, rows, H,
+                                       dtype_code(output_grad.dtype), L.stream),
             "ck_swiglu_backward_mx8",
         )
 
 
-def _halves(t, H: int, size: int):
-    """Addresses of the two halves of a row of 2 H elements: (up, gate)."""
-    first = _ptr(t)
-    return first, None if first is None else first + H * size
+def _unchunked_operands(what: str, whole, half, codes, scales, activation) -> tuple[int, int]:
+    rows, H = _rows_alike(what, half, activation)
+    _rows_alike(what, whole)
+    _mx8_pair(what, codes, scales)
+    lead = half.shape[:-1]
+    if whole.dtype != half.dtype or whole.shape != (*lead, 2 * H) or codes.shape != (*lead, 2, H):
+        raise ValueError(f"{what}: rows of 2 H beside rows of H, codes [..., 2, H]")
+    return rows, H
 
 
 def swiglu_unchunked_forward_mx8(x, output, codes, scales) -> None:
     """x [..., 2 H] = (up | gate); codes [..., 2, H] and scales [..., 2, ceil(H / 32)]: each half has blocks of its own."""
     lib = load_library()
-    _same_dtype(x, "swiglu_unchunked_forward_mx8", output=output)
-    _dense("swiglu_unchunked_forward_mx8", x=x, output=output)
-    _mx8_pair("swiglu_unchunked_forward_mx8", codes, scales)
-    rows, H = _rows_of(output)
-    if x.size(-1) != 2 * H or x.numel() != 2 * output.numel() or codes.numel() != x.numel() or codes.shape[-2:] != (2, H):
-        raise ValueError("swiglu_unchunked_forward_mx8: x [..., 2 H], output [..., H], codes [..., 2, H]")
+    rows, H = _unchunked_operands("swiglu_unchunked_forward_mx8", x, output, codes, scales, None)
+    if rows == 0 or H == 0:
+        return
     with _Launch(x, output, codes, scales) as L:
-        up, gate = _halves(x, H, x.element_size())
-        up_codes, gate_codes = _halves(codes, H, 1)
-        up_scales, gate_scales = _halves(scales, mx8_blocks(H), 1)
+        up, c, s, blocks = _ptr(x), _ptr(codes), _ptr(scales), mx8_blocks(H)
         _check(
-            lib.ck_swiglu_forward_mx8(gate, up, 2 * H, _ptr(output), gate_codes, up_codes, 2 * H, gate_scales, up_scales,
-                                      2 * mx8_blocks(H), rows, H, dtype_code(x.dtype), L.stream),
+            lib.ck_swiglu_forward_mx8(up + H * x.element_size(), up, 2 * H, _ptr(output), c + H, c, 2 * H, s + blocks, s,
+                                      2 * blocks, rows, H, dtype_code(x.dtype), L.stream),
             "ck_swiglu_forward_mx8",
         )
 
 
 def swiglu_unchunked_backward_mx8(codes, scales, output_grad, x_grad, activation=None) -> None:
     lib = load_library()
-    _same_dtype(output_grad, "swiglu_unchunked_backward_mx8", x_grad=x_grad, activation=activation)
-    _dense("swiglu_unchunked_backward_mx8", output_grad=output_grad, x_grad=x_grad, activation=activation)
-    _mx8_pair("swiglu_unchunked_backward_mx8", codes, scales)
-    rows, H = _rows_of(output_grad)
-    if x_grad.size(-1) != 2 * H or x_grad.numel() != 2 * output_grad.numel() or codes.numel() != x_grad.numel() or (
-            codes.shape[-2:] != (2, H)) or (activation is not None and activation.shape != output_grad.shape):
-        raise ValueError("swiglu_unchunked_backward_mx8: output_grad [..., H], x_grad [..., 2 H], codes [..., 2, H]")
+    rows, H = _unchunked_operands("swiglu_unchunked_backward_mx8", x_grad, output_grad, codes, scales, activation)
+    if rows == 0 or H == 0:
+        return
     with _Launch(codes, scales, output_grad, x_grad, activation) as L:
-        up_codes, gate_codes = _halves(codes, H, 1)
-        up_scales, gate_scales = _halves(scales, mx8_blocks(H), 1)
-        up_grad, gate_grad = _halves(x_grad, H, x_grad.element_size())
+        d_up, c, s, blocks = _ptr(x_grad), _ptr(codes), _ptr(scales), mx8_blocks(H)
         _check(
-            lib.ck_swiglu_backward_mx8(gate_codes, up_codes, 2 * H, gate_scales, up_scales, 2 * mx8_blocks(H),
-                                       _ptr(output_grad), gate_grad, up_grad, 2 * H, _ptr(activation), rows, H,
+            lib.ck_swiglu_backward_mx8(c + H, c, 2 * H, s + blocks, s, 2 * blocks, _ptr(output_grad),
+                                       d_up + H * x_grad.element_size(), d_up, 2 * H, _ptr(activation), rows, H,
                                        dtype_code(output_grad.dtype), L.stream),
             "ck_swiglu_backward_mx8",
         )
+
+
+def _norm_vectors(what: str, dtype, B: int, H: int, rstd, *weights) -> None:
+    for t in weights:
+        if t is not None and (t.dtype != dtype or t.numel() != H or not t.is_contiguous()):
+            raise ValueError(f"{what}: weight and its gradient are dense [H] of the rows' dtype")
+    if rstd.dtype != torch.float32 or rstd.numel() != B or not rstd.is_contiguous():
+        raise ValueError(f"{what}: rstd is dense fp32 [rows]")
 
 
 def rmsnorm_forward_mx8(x, residual, weight, output, residual_out, codes, scales, rstd, eps: float) -> None:
     """Rows of x (+ residual, whose sum goes to residual_out) normalised, and kept in 8 bits with their 1 / rms."""
     lib = load_library()
     what = "rmsnorm_forward_mx8"
-    _same_dtype(x, what, residual=residual, weight=weight, output=output, residual_out=residual_out)
-    _dense(what, x=x, residual=residual, weight=weight, output=output, residual_out=residual_out, rstd=rstd)
+    B, H = _rows_alike(what, x, residual, output, residual_out)
+    _norm_vectors(what, x.dtype, B, H, rstd, weight)
     _mx8_pair(what, codes, scales)
-    B, H = _rows_of(x)
-    if (residual is None) != (residual_out is None):
-        raise ValueError(f"{what}: residual and residual_out go together")
-    for t in (residual, output, residual_out, codes):
-        if t is not None and t.shape != x.shape:
-            raise ValueError(f"{what}: all operands have the shape of x")
-    if (weight is not None and weight.numel() != H) or rstd.dtype != torch.float32 or rstd.numel() != B:
-        raise ValueError(f"{what}: weight [H], rstd fp32 [rows]")
+    if codes.shape != x.shape or (residual is None) != (residual_out is None):
+        raise ValueError(f"{what}: codes of the shape of x, residual_out with a residual")
     with _Launch(x, residual, weight, output, residual_out, codes, scales, rstd) as L:
         _check(
             lib.ck_rmsnorm_forward_mx8(_ptr(x), _ptr(residual), _ptr(weight), _ptr(output), _ptr(residual_out),
@@ -1087,8 +1091,9 @@ def rmsnorm_forward_mx8(x, residual, weight, output, residual_out, codes, scales
 
 
 def rmsnorm_backward_mx8_workspace_size(B: int, H: int, device: torch.device) -> int:
+    """Depends on the compute units of the device that is current in the call."""
     lib = load_library()
-    if device.type != "cuda" or device.index == torch.cuda.current_device():
+    if device.type != "cuda" or device.index == torch._C._cuda_getDevice():
         return lib.ck_rmsnorm_backward_mx8_workspace_size(B, H)
     with torch.cuda.device(device):
         return lib.ck_rmsnorm_backward_mx8_workspace_size(B, H)
@@ -1097,17 +1102,11 @@ def rmsnorm_backward_mx8_workspace_size(B: int, H: int, device: torch.device) ->
 def rmsnorm_backward_mx8(codes, scales, weight, output_grad, rstd, sum_grad, x_grad, weight_grad, workspace) -> None:
     lib = load_library()
     what = "rmsnorm_backward_mx8"
-    _same_dtype(output_grad, what, weight=weight, sum_grad=sum_grad, x_grad=x_grad, weight_grad=weight_grad)
-    _dense(what, output_grad=output_grad, weight=weight, sum_grad=sum_grad, x_grad=x_grad, weight_grad=weight_grad, rstd=rstd)
+    B, H = _rows_alike(what, output_grad, sum_grad, x_grad)
+    _norm_vectors(what, output_grad.dtype, B, H, rstd, weight, weight_grad)
     _mx8_pair(what, codes, scales)
-    B, H = _rows_of(output_grad)
-    for t in (sum_grad, x_grad, codes):
-        if t is not None and t.shape != output_grad.shape:
-            raise ValueError(f"{what}: all operands have the shape of output_grad")
-    if (weight is None) != (weight_grad is None) or (weight is not None and (weight.numel() != H or weight_grad.numel() != H)):
-        raise ValueError(f"{what}: weight and weight_grad go together, [H] each")
-    if rstd.dtype != torch.float32 or rstd.numel() != B:
-        raise ValueError(f"{what}: rstd fp32 [rows]")
+    if codes.shape != output_grad.shape or (weight is None) != (weight_grad is None):
+        raise ValueError(f"{what}: codes of the shape of output_grad, weight_grad with a weight")
     with _Launch(codes, scales, weight, output_grad, rstd, sum_grad, x_grad, weight_grad, workspace) as L:
         _check(
             lib.ck_rmsnorm_backward_mx8(

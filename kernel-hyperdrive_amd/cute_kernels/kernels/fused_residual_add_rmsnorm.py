@@ -18,15 +18,7 @@ from ..enums import KernelBackend
 from ..utils import cute_op, ensure_contiguous
 from ._common import check_backend
 from .add import add_tensor_forward_hip
-from .mx8 import new_mx8
-from .rmsnorm import (
-    _backward,
-    _check_mx8_arguments,
-    _check_row_length,
-    _wants_grad,
-    rmsnorm_backward_mx8_hip,
-    rmsnorm_forward_mx8_hip,
-)
+from .rmsnorm import _backward, _check_row_length, _keeps_8bit, rmsnorm_backward_mx8, rmsnorm_forward_mx8
 
 
 def fused_residual_add_rmsnorm_torch(
@@ -139,61 +131,23 @@ class _FusedResidualAddRMSNormMX8_Cute(torch.autograd.Function):
     backward adds the gradient that reaches the returned sum in the same pass, rounded once."""
 
     @staticmethod
-    @ensure_contiguous
     def forward(
         ctx, x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None, eps: float | None
     ) -> tuple[torch.Tensor, torch.Tensor]:
-        assert x.size() == residual.size(), "tensors x and residual should have same shape"
-        assert x.type() == residual.type(), "tensors x and residual should have same dtype"
-        if eps is None:
-            eps = torch.finfo(x.dtype).eps
-        ctx.shape = x.shape
-        rows = x.shape if x.dim() > 1 else (1, x.numel())
-        hidden_size = x.size(-1)
-        num_rows = x.numel() // hidden_size if hidden_size > 0 else 0
-        output = torch.empty_like(x)
-        residual_output = torch.empty_like(x)
-        codes, scales = new_mx8(rows, x.device)
-        rmsnorm_denominator = torch.empty(num_rows, device=x.device, dtype=torch.float32)
-        rmsnorm_forward_mx8_hip(
-            x=x.view(rows),
-            residual=residual.view(rows),
-            weight=weight,
-            output=output.view(rows),
-            residual_output=residual_output.view(rows),
-            codes=codes,
-            scales=scales,
-            rmsnorm_denominator=rmsnorm_denominator,
-            eps=eps,
+        output, residual_output, kept = rmsnorm_forward_mx8(
+            x.contiguous(), residual.contiguous(), None if weight is None else weight.contiguous(), eps
         )
-        ctx.save_for_backward(codes, scales, weight, rmsnorm_denominator)
+        ctx.save_for_backward(*kept)
         ctx.set_materialize_grads(False)
         return output, residual_output
 
     @staticmethod
-    @ensure_contiguous
     def backward(ctx, output_grad: torch.Tensor | None, residual_output_grad: torch.Tensor | None):
-        codes, scales, weight, rmsnorm_denominator = ctx.saved_tensors
-        weight_grad = None if weight is None else torch.empty_like(weight)
         if output_grad is None:
             # only the sum was used: the normalisation has no gradient
-            weight_grad = None if weight is None else torch.zeros_like(weight)
-            return residual_output_grad, residual_output_grad, weight_grad, None
-        output_grad = output_grad.view(codes.shape)
-        if residual_output_grad is not None:
-            residual_output_grad = residual_output_grad.view(codes.shape)
-        x_grad = torch.empty_like(output_grad)
-        rmsnorm_backward_mx8_hip(
-            codes=codes,
-            scales=scales,
-            weight=weight,
-            output_grad=output_grad,
-            rmsnorm_denominator=rmsnorm_denominator,
-            sum_grad=residual_output_grad,
-            x_grad=x_grad,
-            weight_grad=weight_grad,
-        )
-        x_grad = x_grad.view(ctx.shape)
+            weight = ctx.saved_tensors[2]
+            return residual_output_grad, residual_output_grad, None if weight is None else torch.zeros_like(weight), None
+        x_grad, weight_grad = rmsnorm_backward_mx8(ctx.saved_tensors, output_grad, residual_output_grad)
         # the sum hands the same gradient to both of its terms
         return x_grad, x_grad, weight_grad, None
 
@@ -209,10 +163,10 @@ def fused_residual_add_rmsnorm_cute(
     checkpoint_8bit: bool = False,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """``(rmsnorm(x + residual, weight, eps), x + residual)``; arguments as in ``rmsnorm_cute``."""
-    if checkpoint_8bit:
-        _check_mx8_arguments(x, weight, memory_efficient)
-        if _wants_grad(x, residual, weight):
-            return _FusedResidualAddRMSNormMX8_Cute.apply(x, residual, weight, eps)
+    if checkpoint_8bit and _keeps_8bit(x, weight, memory_efficient, residual):
+        assert x.shape == residual.shape, "tensors x and residual should have same shape"
+        assert x.dtype == residual.dtype, "tensors x and residual should have same dtype"
+        return _FusedResidualAddRMSNormMX8_Cute.apply(x, residual, weight, eps)
     return _FusedResidualAddRMSNorm_Cute.apply(
         x, residual, weight, eps, memory_efficient, kernel_backend_forward, kernel_backend_backward
     )

@@ -265,77 +265,91 @@ def rmsnorm_backward_mx8_hip(
 ) -> None:
     workspace = None
     if weight is not None:
-        hidden_size = output_grad.size(-1)
-        num_rows = output_grad.numel() // hidden_size if hidden_size > 0 else 0
-        nbytes = _C.rmsnorm_backward_mx8_workspace_size(num_rows, hidden_size, output_grad.device)
-        workspace = torch.empty(max(nbytes, 16), device=output_grad.device, dtype=torch.uint8)
+        # fp32 partial rows of the dweight sum; taken from torch's caching allocator
+        nbytes = _C.rmsnorm_backward_mx8_workspace_size(rmsnorm_denominator.numel(), weight.numel(), weight.device)
+        workspace = torch.empty(max(nbytes, 16), device=weight.device, dtype=torch.uint8)
     _C.rmsnorm_backward_mx8(
         codes, scales, weight, output_grad, rmsnorm_denominator, sum_grad, x_grad, weight_grad, workspace
     )
 
 
-def _check_mx8_arguments(x: torch.Tensor, weight: torch.Tensor | None, memory_efficient: bool) -> None:
+def _keeps_8bit(x: torch.Tensor, weight: torch.Tensor | None, memory_efficient: bool, *others: torch.Tensor) -> bool:
+    """Checks the arguments of a call with ``checkpoint_8bit``; whether it has a backward to keep anything for."""
     if weight is not None:
         assert weight.dim() == 1, "weight should be 1D"
-        assert weight.size(-1) == x.size(-1), "hidden size for x and weight tensor is different"
-        assert weight.type() == x.type(), "tensors weight and y should have same dtype"
+        assert weight.size(0) == x.size(-1), "hidden size for x and weight tensor is different"
+        assert weight.dtype == x.dtype, "tensors weight and y should have same dtype"
     if memory_efficient:
         # 1 / rms is that of the exact row: it cannot be had again from the kept one
         raise ValueError("checkpoint_8bit saves 1 / rms and does not go with memory_efficient")
     _check_row_length(x.size(-1))
+    if not torch.is_grad_enabled():
+        return False
+    return x.requires_grad or (weight is not None and weight.requires_grad) or any(t.requires_grad for t in others)
+
+
+def rmsnorm_forward_mx8(x, residual, weight, eps):
+    """(output, x + residual or None, what the backward needs) of contiguous operands."""
+    if eps is None:
+        eps = torch.finfo(x.dtype).eps
+    output = torch.empty_like(x)
+    residual_output = None if residual is None else torch.empty_like(x)
+    rows = x
+    if x.dim() == 1:
+        rows, residual = x.unsqueeze(0), None if residual is None else residual.unsqueeze(0)
+    codes, scales = new_mx8(rows.shape, x.device)
+    hidden_size = x.size(-1)
+    num_rows = x.numel() // hidden_size if hidden_size > 0 else 0
+    rmsnorm_denominator = torch.empty(num_rows, device=x.device, dtype=torch.float32)
+    rmsnorm_forward_mx8_hip(
+        rows,
+        residual,
+        weight,
+        output.view(rows.shape) if rows is not x else output,
+        residual_output.view(rows.shape) if rows is not x and residual is not None else residual_output,
+        codes,
+        scales,
+        rmsnorm_denominator,
+        eps,
+    )
+    return output, residual_output, (codes, scales, weight, rmsnorm_denominator)
+
+
+def rmsnorm_backward_mx8(kept, output_grad, sum_grad):
+    """(gradient of the normalised rows, plus ``sum_grad`` where there is one, rounded once; the weight's)."""
+    codes, scales, weight, rmsnorm_denominator = kept
+    output_grad = output_grad.contiguous()
+    if sum_grad is not None:
+        sum_grad = sum_grad.contiguous()
+    x_grad = torch.empty_like(output_grad)
+    weight_grad = None if weight is None else torch.empty_like(weight)
+    is_1d = output_grad.dim() == 1
+    rmsnorm_backward_mx8_hip(
+        codes,
+        scales,
+        weight,
+        output_grad.unsqueeze(0) if is_1d else output_grad,
+        rmsnorm_denominator,
+        sum_grad.unsqueeze(0) if is_1d and sum_grad is not None else sum_grad,
+        x_grad.unsqueeze(0) if is_1d else x_grad,
+        weight_grad,
+    )
+    return x_grad, weight_grad
 
 
 class _RMSNormMX8_Cute(torch.autograd.Function):
     """As ``_RMSNorm_Cute``, with x saved in 8 bits (see mx8.py) by the forward's own pass; 1 / rms is saved as well."""
 
     @staticmethod
-    @ensure_contiguous
     def forward(ctx, x: torch.Tensor, weight: torch.Tensor | None, eps: float | None) -> torch.Tensor:
-        if eps is None:
-            eps = torch.finfo(x.dtype).eps
-        ctx.shape = x.shape
-        rows = x.shape if x.dim() > 1 else (1, x.numel())
-        hidden_size = x.size(-1)
-        num_rows = x.numel() // hidden_size if hidden_size > 0 else 0
-        output = torch.empty_like(x)
-        codes, scales = new_mx8(rows, x.device)
-        rmsnorm_denominator = torch.empty(num_rows, device=x.device, dtype=torch.float32)
-        rmsnorm_forward_mx8_hip(
-            x=x.view(rows),
-            residual=None,
-            weight=weight,
-            output=output.view(rows),
-            residual_output=None,
-            codes=codes,
-            scales=scales,
-            rmsnorm_denominator=rmsnorm_denominator,
-            eps=eps,
-        )
-        ctx.save_for_backward(codes, scales, weight, rmsnorm_denominator)
+        output, _, kept = rmsnorm_forward_mx8(x.contiguous(), None, None if weight is None else weight.contiguous(), eps)
+        ctx.save_for_backward(*kept)
         return output
 
     @staticmethod
-    @ensure_contiguous
     def backward(ctx, output_grad: torch.Tensor):
-        codes, scales, weight, rmsnorm_denominator = ctx.saved_tensors
-        output_grad = output_grad.view(codes.shape)
-        x_grad = torch.empty_like(output_grad)
-        weight_grad = None if weight is None else torch.empty_like(weight)
-        rmsnorm_backward_mx8_hip(
-            codes=codes,
-            scales=scales,
-            weight=weight,
-            output_grad=output_grad,
-            rmsnorm_denominator=rmsnorm_denominator,
-            sum_grad=None,
-            x_grad=x_grad,
-            weight_grad=weight_grad,
-        )
-        return x_grad.view(ctx.shape), weight_grad, None
-
-
-def _wants_grad(*tensors: torch.Tensor | None) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+        x_grad, weight_grad = rmsnorm_backward_mx8(ctx.saved_tensors, output_grad, None)
+        return x_grad, weight_grad, None
 
 
 def rmsnorm_cute(
@@ -353,10 +367,8 @@ def rmsnorm_cute(
 ) -> torch.Tensor:
     """``checkpoint_8bit``: keep x for the backward in 8 bits (see mx8.py); the output is that of the exact rows, the gradients
     are those at the kept rows with the exact rows' 1 / rms.  Not with ``memory_efficient``; the tunables have no meaning there."""
-    if checkpoint_8bit:
-        _check_mx8_arguments(x, weight, memory_efficient)
-        if _wants_grad(x, weight):
-            return _RMSNormMX8_Cute.apply(x, weight, eps)
+    if checkpoint_8bit and _keeps_8bit(x, weight, memory_efficient):
+        return _RMSNormMX8_Cute.apply(x, weight, eps)
     return _RMSNorm_Cute.apply(
         x,
         weight,

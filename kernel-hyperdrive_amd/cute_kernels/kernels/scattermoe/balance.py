@@ -72,9 +72,7 @@ class _MoEBalanceLoss_Cute(torch.autograd.Function):
         z = torch.empty((), dtype=torch.float32, device=device)
         counts = torch.empty(logits.size(1), dtype=torch.int32, device=device)
         stats = torch.empty(2, dtype=torch.int32, device=device)
-        moe_balance_loss_forward_hip(
-            logits=logits, selected=selected, mask=mask, balance=balance, z=z, counts=counts, stats=stats
-        )
+        moe_balance_loss_forward_hip(logits, selected, mask, balance, z, counts, stats)
         ctx.save_for_backward(logits, mask, counts, stats)
         ctx.top_k = selected.size(1)
         ctx.mark_non_differentiable(counts)
@@ -87,16 +85,7 @@ class _MoEBalanceLoss_Cute(torch.autograd.Function):
         if balance_grad is None and z_grad is None:
             return None, None, None
         d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        moe_balance_loss_backward_hip(
-            logits=logits,
-            mask=mask,
-            counts=counts,
-            stats=stats,
-            balance_grad=balance_grad,
-            z_grad=z_grad,
-            d_logits=d_logits,
-            top_k=ctx.top_k,
-        )
+        moe_balance_loss_backward_hip(logits, mask, counts, stats, balance_grad, z_grad, d_logits, ctx.top_k)
         return d_logits, None, None
 
 
@@ -115,7 +104,7 @@ def moe_balance_loss_cute(
     token both losses are 0.  A token whose logits are all -inf or the type's lowest value has no probabilities: it counts in N
     and adds nothing."""
     E = router_logits.size(-1)
-    logits = router_logits.reshape(-1, E)
+    logits = router_logits if router_logits.dim() == 2 else router_logits.reshape(-1, E)
     if (E > 1 and logits.stride(1) != 1) or (logits.size(0) > 1 and logits.stride(0) < E):
         logits = logits.contiguous()
     if selected_experts is None:
@@ -132,7 +121,9 @@ def moe_balance_loss_cute(
             )
         if top_k is not None and selected_experts.size(-1) != top_k:
             raise ValueError("moe_balance_loss_cute: top_k is not the number of selected experts")
-        selected_experts = _C._index_i64(selected_experts, "selected_experts").view(-1, selected_experts.size(-1))
+        selected_experts = _C._index_i64(selected_experts, "selected_experts")
+        if selected_experts.dim() != 2:
+            selected_experts = selected_experts.view(-1, selected_experts.size(-1))
     if token_mask is not None:
         if token_mask.dtype != torch.bool or token_mask.shape != router_logits.shape[:-1]:
             raise ValueError("moe_balance_loss_cute: token_mask is one bool per token")

@@ -97,78 +97,41 @@ class _Swiglu_Cute(torch.autograd.Function):
         return gate_grad, up_grad, None, None, None, None
 
 
-@cute_op(
-    f"{LIBRARY_NAME}::swiglu_forward_mx8_hip",
-    mutates_args={"output", "gate_codes", "gate_scales", "up_codes", "up_scales"},
-)
+@cute_op(f"{LIBRARY_NAME}::swiglu_forward_mx8_hip", mutates_args={"output", "codes", "scales"})
 def swiglu_forward_mx8_hip(
-    gate: torch.Tensor,
-    up: torch.Tensor,
-    output: torch.Tensor,
-    gate_codes: torch.Tensor,
-    gate_scales: torch.Tensor,
-    up_codes: torch.Tensor,
-    up_scales: torch.Tensor,
+    gate: torch.Tensor, up: torch.Tensor, output: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor
 ) -> None:
-    _C.swiglu_forward_mx8(gate, up, output, gate_codes, gate_scales, up_codes, up_scales)
+    _C.swiglu_forward_mx8(gate, up, output, codes, scales)
 
 
 @cute_op(f"{LIBRARY_NAME}::swiglu_backward_mx8_hip", mutates_args={"gate_grad", "up_grad"})
 def swiglu_backward_mx8_hip(
-    gate_codes: torch.Tensor,
-    gate_scales: torch.Tensor,
-    up_codes: torch.Tensor,
-    up_scales: torch.Tensor,
-    output_grad: torch.Tensor,
-    gate_grad: torch.Tensor,
-    up_grad: torch.Tensor,
+    codes: torch.Tensor, scales: torch.Tensor, output_grad: torch.Tensor, gate_grad: torch.Tensor, up_grad: torch.Tensor
 ) -> None:
-    _C.swiglu_backward_mx8(gate_codes, gate_scales, up_codes, up_scales, output_grad, gate_grad, up_grad)
+    _C.swiglu_backward_mx8(codes, scales, output_grad, gate_grad, up_grad)
 
 
 class _SwigluMX8_Cute(torch.autograd.Function):
-    """As ``_Swiglu_Cute``, with gate and up saved in 8 bits (see mx8.py) by the forward's own pass."""
+    """As ``_Swiglu_Cute``, with gate and up saved in 8 bits (see mx8.py) by the forward's own pass: codes and scale bytes of
+    the two behind one another."""
 
     @staticmethod
-    @ensure_contiguous
     def forward(ctx, gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
-        assert gate.size() == up.size(), "tensors gate and up should have same shape"
-        assert gate.type() == up.type(), "tensors gate and up should have same dtype"
-
-        ctx.shape = gate.shape
-        rows = gate.shape if gate.dim() > 1 else (1, gate.numel())
+        gate, up = gate.contiguous(), up.contiguous()
         output = torch.empty_like(gate)
-        gate_codes, gate_scales = new_mx8(rows, gate.device)
-        up_codes, up_scales = new_mx8(rows, gate.device)
-        swiglu_forward_mx8_hip(
-            gate=gate.view(rows),
-            up=up.view(rows),
-            output=output.view(rows),
-            gate_codes=gate_codes,
-            gate_scales=gate_scales,
-            up_codes=up_codes,
-            up_scales=up_scales,
-        )
-        ctx.save_for_backward(gate_codes, gate_scales, up_codes, up_scales)
+        codes, scales = new_mx8((2, *gate.shape), gate.device)
+        swiglu_forward_mx8_hip(gate, up, output, codes, scales)
+        ctx.save_for_backward(codes, scales)
         return output
 
     @staticmethod
-    @ensure_contiguous
     def backward(ctx, output_grad: torch.Tensor):
-        gate_codes, gate_scales, up_codes, up_scales = ctx.saved_tensors
-        output_grad = output_grad.view(gate_codes.shape)
+        codes, scales = ctx.saved_tensors
+        output_grad = output_grad.contiguous()
         gate_grad = torch.empty_like(output_grad)
         up_grad = torch.empty_like(output_grad)
-        swiglu_backward_mx8_hip(
-            gate_codes=gate_codes,
-            gate_scales=gate_scales,
-            up_codes=up_codes,
-            up_scales=up_scales,
-            output_grad=output_grad,
-            gate_grad=gate_grad,
-            up_grad=up_grad,
-        )
-        return gate_grad.view(ctx.shape), up_grad.view(ctx.shape)
+        swiglu_backward_mx8_hip(codes, scales, output_grad, gate_grad, up_grad)
+        return gate_grad, up_grad
 
 
 def swiglu_cute(
@@ -183,6 +146,8 @@ def swiglu_cute(
     """``checkpoint_8bit``: keep gate and up for the backward in 8 bits (see mx8.py); the output is that of the exact
     inputs, the gradients are those at the kept values.  The other tunables have no meaning there."""
     if checkpoint_8bit and torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad):
+        assert gate.shape == up.shape, "tensors gate and up should have same shape"
+        assert gate.dtype == up.dtype, "tensors gate and up should have same dtype"
         return _SwigluMX8_Cute.apply(gate, up)
     return _Swiglu_Cute.apply(
         gate, up, kernel_backend_forward, kernel_backend_backward, BLOCK_SIZE_forward, BLOCK_SIZE_backward

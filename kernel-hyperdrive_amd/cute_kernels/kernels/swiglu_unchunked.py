@@ -120,22 +120,23 @@ class _SwigluUnchunkedMX8_Cute(torch.autograd.Function):
     """As ``_SwigluUnchunked_Cute``, with x saved in 8 bits (see mx8.py; each half of a row has blocks of its own)."""
 
     @staticmethod
-    @ensure_contiguous
     def forward(ctx, x: torch.Tensor) -> torch.Tensor:
-        h = divide_if_divisible(x.size(-1), 2, "last dimension of x must be even")
-        output = torch.empty(*x.size()[:-1], h, device=x.device, dtype=x.dtype)
-        codes, scales = new_mx8((*x.size()[:-1], 2, h), x.device)
-        swiglu_unchunked_forward_mx8_hip(x=x, output=output, codes=codes, scales=scales)
+        x = x.contiguous()
+        *lead, H = x.shape
+        h = divide_if_divisible(H, 2, "last dimension of x must be even")
+        output = torch.empty((*lead, h), device=x.device, dtype=x.dtype)
+        codes, scales = new_mx8((*lead, 2, h), x.device)
+        swiglu_unchunked_forward_mx8_hip(x, output, codes, scales)
         ctx.save_for_backward(codes, scales)
         return output
 
     @staticmethod
-    @ensure_contiguous
     def backward(ctx, output_grad: torch.Tensor):
         codes, scales = ctx.saved_tensors
-        h = output_grad.size(-1)
-        x_grad = torch.empty(*output_grad.size()[:-1], 2 * h, device=output_grad.device, dtype=output_grad.dtype)
-        swiglu_unchunked_backward_mx8_hip(codes=codes, scales=scales, output_grad=output_grad, x_grad=x_grad)
+        output_grad = output_grad.contiguous()
+        *lead, h = output_grad.shape
+        x_grad = torch.empty((*lead, 2 * h), device=output_grad.device, dtype=output_grad.dtype)
+        swiglu_unchunked_backward_mx8_hip(codes, scales, output_grad, x_grad)
         return x_grad
 
 
