@@ -379,7 +379,8 @@ int ck_moe_balance_loss_backward(const void* logits, int64_t ld, const void* mas
  *                    is summed through `workspace` without atomics.
  * ck_moe_combine_backward_gates_mx8
  *                    ck_moe_combine_backward_gates with the expert outputs [tokens, k, H] in 8 bits.
- * rows * 4 * ceil(H / 32) < 2^31 for the element-wise ones, H <= 65536 and B < 2^31 for RMSNorm.
+ * Rows of 16-byte pieces, whole blocks each: fewer than 2^31 of them for the element-wise ones; H <= 65536 and B < 2^31
+ * for RMSNorm.
  * ------------------------------------------------------------------------------------------- */
 int ck_mx8_quantize(const void* x, void* codes, void* scales, int64_t rows, int64_t H, int dtype, void* stream);
 int ck_mx8_dequantize(const void* codes, const void* scales, const int64_t* index, int64_t fan, int64_t source_rows,
@@ -392,7 +393,7 @@ int ck_swiglu_backward_mx8(const void* gate_codes, const void* up_codes, int64_t
                            int64_t ldx, void* activation, int64_t rows, int64_t H, int dtype, void* stream);
 int ck_rmsnorm_forward_mx8(const void* x, const void* residual, const void* weight, void* output, void* residual_out,
                            void* codes, void* scales, float* rstd, int64_t B, int64_t H, float eps, int dtype, void* stream);
-int64_t ck_rmsnorm_backward_mx8_workspace_size(int64_t B, int64_t H);
+int64_t ck_rmsnorm_backward_mx8_workspace_size(int64_t B, int64_t H, int dtype);
 int ck_rmsnorm_backward_mx8(const void* codes, const void* scales, const void* weight, const void* output_grad,
                             const float* rstd, const void* sum_grad, void* x_grad, void* weight_grad, void* workspace,
                             int64_t workspace_bytes, int64_t B, int64_t H, int dtype, void* stream);

@@ -15,6 +15,7 @@
 namespace ck {
 
 constexpr int kBalanceMaxExperts = 1024;
+constexpr int kPiece = 8;  // experts a lane holds side by side
 
 template <int LPT>
 __device__ __forceinline__ float group_max(float v) {
@@ -159,9 +160,9 @@ __global__ void __launch_bounds__(WAVES * CK_WAVE)
         for (int c = 0; c < CHUNKS; ++c) {
             const int col = first + c * LPT * kPiece;
             const int left = E - col, size = left >= kPiece ? kPiece : (left > 0 ? left : 0);
-            Piece<T> row;
+            Piece<T, kPiece> row;
             row.clear();
-            if (real && size > 0) row = load_piece<T, VEC, false>(logits + t * ld + col, size);
+            if (real && size > 0) row = load_piece<T, kPiece, VEC, false>(logits + t * ld + col, size);
 #pragma unroll
             for (int j = 0; j < kPiece; ++j) v[c][j] = row.up(j);
         }
@@ -295,9 +296,9 @@ __global__ void __launch_bounds__(256)
         for (int c = 0; c < CHUNKS; ++c) {
             const int col = first + c * LPT * kPiece;
             const int left = E - col, size = left >= kPiece ? kPiece : (left > 0 ? left : 0);
-            Piece<T> row;
+            Piece<T, kPiece> row;
             row.clear();
-            if (real && size > 0) row = load_piece<T, VEC, false>(logits + t * ld + col, size);
+            if (real && size > 0) row = load_piece<T, kPiece, VEC, false>(logits + t * ld + col, size);
 #pragma unroll
             for (int j = 0; j < kPiece; ++j) v[c][j] = row.up(j);
         }
@@ -313,10 +314,10 @@ __global__ void __launch_bounds__(256)
         for (int c = 0; c < CHUNKS; ++c) {
             const int col = first + c * LPT * kPiece;
             const int left = E - col, size = left >= kPiece ? kPiece : (left > 0 ? left : 0);
-            Piece<T> o;
+            Piece<T, kPiece> o;
 #pragma unroll
             for (int j = 0; j < kPiece; ++j) o.put(j, real ? v[c][j] * (a[c][j] + shift) : 0.f);
-            if (t < tokens && size > 0) store_piece<T, VEC>(o, d_logits + t * E + col, size);
+            if (t < tokens && size > 0) store_piece<T, kPiece, VEC>(o, d_logits + t * E + col, size);
         }
     }
 }

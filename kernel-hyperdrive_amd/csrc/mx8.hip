@@ -1,41 +1,44 @@
 // Activations in 8 bits (ck_mx8.h) for gfx950: writing and reading them, SwiGLU forward with its inputs kept in 8 bits and
 // its backward from them, and the routing weights' gradient from expert outputs kept in 8 bits.
-// HBM-bound streaming kernels in the manner of swiglu.hip: a lane moves pieces of eight elements, several in flight, fp32
+// HBM-bound streaming kernels in the manner of swiglu.hip: a lane moves 16-byte pieces, several in flight, fp32
 // math, one rounding on store.
 #include "ck_mx8.h"
 
 namespace ck {
 
 constexpr int kMxThreads = 256;
-constexpr int kMxUnroll = 4;  // pieces per lane
+// Pieces per lane of the two that move one tensor; the SwiGLU kernels move two or three and take one.  16384 x 4096 bf16:
+// quantize 35.5 / 32.5 / 34.8 us with 1 / 2 / 4 pieces, dequantize 33.5 / 33.7 / 34.7; SwiGLU backward 85.0 / 87.3 with 1 / 2.
+constexpr int kMxUnroll = 2;
 
 template <typename T, int MODE>
 __global__ void __launch_bounds__(kMxThreads)
     mx8_quantize_kernel(const typename T::storage_t* __restrict__ x, int8_t* __restrict__ codes, uint8_t* __restrict__ scales,
                         MxShape shape) {
+    constexpr int N = kMxPiece<T>, LANES = kMxLanes<T>;
     constexpr bool VEC = MODE != kMxAny;
-    const int64_t blocks = shape.per_row / kMxQuad;
+    const int64_t blocks = shape.per_row / LANES;
     const uint32_t base = blockIdx.x * (kMxThreads * kMxUnroll) + threadIdx.x;
-    Piece<T> in[kMxUnroll];
+    Piece<T, N> in[kMxUnroll];
 #pragma unroll
     for (int i = 0; i < kMxUnroll; ++i) {
         const uint32_t p = base + i * kMxThreads;
-        const MxAt a = mx_at<MODE>(shape, p);
-        if (mx_has<MODE>(shape, p, a)) in[i] = load_piece<T, VEC>(x + a.row * shape.h + a.col, a.n);
+        const MxAt a = mx_at<N, MODE>(shape, p);
+        if (mx_has<MODE>(shape, p, a)) in[i] = load_piece<T, N, VEC>(x + a.row * shape.h + a.col, a.n);
         else in[i].clear();
     }
 #pragma unroll
     for (int i = 0; i < kMxUnroll; ++i) {
         const uint32_t p = base + i * kMxThreads;
-        const MxAt a = mx_at<MODE>(shape, p);
-        float v[kMxPiece];
+        const MxAt a = mx_at<N, MODE>(shape, p);
+        float v[N];
 #pragma unroll
-        for (int j = 0; j < kMxPiece; ++j) v[j] = in[i].up(j);
+        for (int j = 0; j < N; ++j) v[j] = in[i].up(j);
         uint32_t scale;
-        const MxCodes c = mx_encode(v, scale);
+        const MxCodes<N> c = mx_encode(v, scale);
         if (mx_has<MODE>(shape, p, a)) {
-            store_codes<VEC>(c, codes + a.row * shape.h + a.col, a.n);
-            if (threadIdx.x % kMxQuad == 0) scales[a.row * blocks + a.block] = (uint8_t)scale;
+            store_codes<N, VEC>(c, codes + a.row * shape.h + a.col, a.n);
+            if (threadIdx.x % LANES == 0) scales[a.row * blocks + a.block] = (uint8_t)scale;
         }
     }
 }
@@ -57,21 +60,22 @@ __global__ void __launch_bounds__(kMxThreads)
     mx8_dequantize_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                           const int64_t* __restrict__ index, int64_t fan, int64_t source_rows,
                           typename T::storage_t* __restrict__ out, MxShape shape) {
+    constexpr int N = kMxPiece<T>, LANES = kMxLanes<T>;
     constexpr bool VEC = MODE != kMxAny;
-    const int64_t blocks = shape.per_row / kMxQuad;
+    const int64_t blocks = shape.per_row / LANES;
     const uint32_t base = blockIdx.x * (kMxThreads * kMxUnroll) + threadIdx.x;
-    MxCodes in[kMxUnroll];
+    MxCodes<N> in[kMxUnroll];
     uint32_t scale[kMxUnroll];
 #pragma unroll
     for (int i = 0; i < kMxUnroll; ++i) {
         const uint32_t p = base + i * kMxThreads;
-        const MxAt a = mx_at<MODE>(shape, p);
-        in[i].w[0] = in[i].w[1] = 0;
+        const MxAt a = mx_at<N, MODE>(shape, p);
+        in[i] = MxCodes<N>{};
         scale[i] = 7;
         if (mx_has<MODE>(shape, p, a)) {
             const int64_t row = GATHER ? index[a.row] / fan : a.row;
             if (!GATHER || (row >= 0 && row < source_rows)) {
-                in[i] = load_codes<VEC>(codes + row * shape.h + a.col, a.n);
+                in[i] = load_codes<N, VEC>(codes + row * shape.h + a.col, a.n);
                 scale[i] = scales[row * blocks + a.block];
             }
         }
@@ -79,16 +83,16 @@ __global__ void __launch_bounds__(kMxThreads)
 #pragma unroll
     for (int i = 0; i < kMxUnroll; ++i) {
         const uint32_t p = base + i * kMxThreads;
-        const MxAt a = mx_at<MODE>(shape, p);
-        float v[kMxPiece];
+        const MxAt a = mx_at<N, MODE>(shape, p);
+        float v[N];
         mx_decode(in[i], mx_step(scale[i]), v);
         if (mx_has<MODE>(shape, p, a)) {
-            Piece<T> o;
+            Piece<T, N> o;
 #pragma unroll
-            for (int j = 0; j < kMxPiece; ++j) {
+            for (int j = 0; j < N; ++j) {
                 o.put(j, mx_limit<T>(v[j]));
             }
-            store_piece<T, VEC>(o, out + a.row * shape.h + a.col, a.n);
+            store_piece<T, N, VEC>(o, out + a.row * shape.h + a.col, a.n);
         }
     }
 }
@@ -106,44 +110,35 @@ __global__ void __launch_bounds__(kMxThreads)
                           typename T::storage_t* __restrict__ out, int8_t* __restrict__ gate_codes,
                           int8_t* __restrict__ up_codes, uint8_t* __restrict__ gate_scales, uint8_t* __restrict__ up_scales,
                           MxStrides ld, MxShape shape) {
+    constexpr int N = kMxPiece<T>, LANES = kMxLanes<T>;
     constexpr bool VEC = MODE != kMxAny;
-    constexpr int kUnroll = 2;  // two tensors: as many bytes in flight as the one-tensor kernels
-    const uint32_t base = blockIdx.x * (kMxThreads * kUnroll) + threadIdx.x;
-    Piece<T> g[kUnroll], u[kUnroll];
-#pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-        const uint32_t p = base + i * kMxThreads;
-        const MxAt a = mx_at<MODE>(shape, p);
-        if (mx_has<MODE>(shape, p, a)) {
-            g[i] = load_piece<T, VEC>(gate + a.row * ld.x + a.col, a.n);
-            u[i] = load_piece<T, VEC>(up + a.row * ld.x + a.col, a.n);
-        } else {
-            g[i].clear();
-            u[i].clear();
-        }
+    const uint32_t p = blockIdx.x * kMxThreads + threadIdx.x;
+    const MxAt a = mx_at<N, MODE>(shape, p);
+    const bool has = mx_has<MODE>(shape, p, a);
+    Piece<T, N> g, u, y;
+    if (has) {
+        g = load_piece<T, N, VEC>(gate + a.row * ld.x + a.col, a.n);
+        u = load_piece<T, N, VEC>(up + a.row * ld.x + a.col, a.n);
+    } else {
+        g.clear();
+        u.clear();
     }
+    float gv[N], uv[N];
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-        const uint32_t p = base + i * kMxThreads;
-        const MxAt a = mx_at<MODE>(shape, p);
-        float gv[kMxPiece], uv[kMxPiece];
-        Piece<T> y;
-#pragma unroll
-        for (int j = 0; j < kMxPiece; ++j) {
-            gv[j] = g[i].up(j);
-            uv[j] = u[i].up(j);
-            y.put(j, swiglu_fwd_1<T>(gv[j], uv[j]));
-        }
-        uint32_t gs, us;
-        const MxCodes gc = mx_encode(gv, gs), uc = mx_encode(uv, us);
-        if (mx_has<MODE>(shape, p, a)) {
-            store_piece<T, VEC>(y, out + a.row * shape.h + a.col, a.n);
-            store_codes<VEC>(gc, gate_codes + a.row * ld.codes + a.col, a.n);
-            store_codes<VEC>(uc, up_codes + a.row * ld.codes + a.col, a.n);
-            if (threadIdx.x % kMxQuad == 0) {
-                gate_scales[a.row * ld.scales + a.block] = (uint8_t)gs;
-                up_scales[a.row * ld.scales + a.block] = (uint8_t)us;
-            }
+    for (int j = 0; j < N; ++j) {
+        gv[j] = g.up(j);
+        uv[j] = u.up(j);
+        y.put(j, swiglu_fwd_1<T>(gv[j], uv[j]));
+    }
+    uint32_t gs, us;
+    const MxCodes<N> gc = mx_encode(gv, gs), uc = mx_encode(uv, us);
+    if (has) {
+        store_piece<T, N, VEC>(y, out + a.row * shape.h + a.col, a.n);
+        store_codes<N, VEC>(gc, gate_codes + a.row * ld.codes + a.col, a.n);
+        store_codes<N, VEC>(uc, up_codes + a.row * ld.codes + a.col, a.n);
+        if (threadIdx.x % LANES == 0) {
+            gate_scales[a.row * ld.scales + a.block] = (uint8_t)gs;
+            up_scales[a.row * ld.scales + a.block] = (uint8_t)us;
         }
     }
 }
@@ -168,45 +163,27 @@ __global__ void __launch_bounds__(kMxThreads)
                           const typename T::storage_t* __restrict__ dy, typename T::storage_t* __restrict__ dgate,
                           typename T::storage_t* __restrict__ dup, typename T::storage_t* __restrict__ act, MxStrides ld,
                           MxShape shape) {
+    constexpr int N = kMxPiece<T>;
     constexpr bool VEC = MODE != kMxAny;
-    constexpr int kUnroll = 2;
-    const uint32_t base = blockIdx.x * (kMxThreads * kUnroll) + threadIdx.x;
-    MxCodes gc[kUnroll], uc[kUnroll];
-    uint32_t gs[kUnroll], us[kUnroll];
-    Piece<T> d[kUnroll];
+    const uint32_t p = blockIdx.x * kMxThreads + threadIdx.x;
+    const MxAt a = mx_at<N, MODE>(shape, p);
+    if (!mx_has<MODE>(shape, p, a)) return;
+    const MxCodes<N> gc = load_codes<N, VEC>(gate_codes + a.row * ld.codes + a.col, a.n);
+    const MxCodes<N> uc = load_codes<N, VEC>(up_codes + a.row * ld.codes + a.col, a.n);
+    const float gs = mx_step(gate_scales[a.row * ld.scales + a.block]), us = mx_step(up_scales[a.row * ld.scales + a.block]);
+    const Piece<T, N> d = load_piece<T, N, VEC>(dy + a.row * shape.h + a.col, a.n);
+    Piece<T, N> og, ou, oa;
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-        const uint32_t p = base + i * kMxThreads;
-        const MxAt a = mx_at<MODE>(shape, p);
-        if (mx_has<MODE>(shape, p, a)) {
-            gc[i] = load_codes<VEC>(gate_codes + a.row * ld.codes + a.col, a.n);
-            uc[i] = load_codes<VEC>(up_codes + a.row * ld.codes + a.col, a.n);
-            gs[i] = gate_scales[a.row * ld.scales + a.block];
-            us[i] = up_scales[a.row * ld.scales + a.block];
-            d[i] = load_piece<T, VEC>(dy + a.row * shape.h + a.col, a.n);
-        }
+    for (int j = 0; j < N; ++j) {
+        const float g = mx_code(gc, j) * gs, u = mx_code(uc, j) * us, dy1 = d.up(j);
+        const float s = mx_sigmoid<T>(g), gsig = g * s;
+        og.put(j, dy1 * u * (s + gsig * (1.0f - s)));
+        ou.put(j, dy1 * gsig);
+        if (ACT) oa.put(j, u * gsig);
     }
-#pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-        const uint32_t p = base + i * kMxThreads;
-        const MxAt a = mx_at<MODE>(shape, p);
-        if (mx_has<MODE>(shape, p, a)) {
-            float g[kMxPiece], u[kMxPiece];
-            mx_decode(gc[i], mx_step(gs[i]), g);
-            mx_decode(uc[i], mx_step(us[i]), u);
-            Piece<T> og, ou, oa;
-#pragma unroll
-            for (int j = 0; j < kMxPiece; ++j) {
-                const float dy1 = d[i].up(j), s = mx_sigmoid<T>(g[j]), gs = g[j] * s;
-                og.put(j, dy1 * u[j] * (s + gs * (1.0f - s)));
-                ou.put(j, dy1 * gs);
-                if (ACT) oa.put(j, u[j] * gs);
-            }
-            store_piece<T, VEC>(og, dgate + a.row * ld.x + a.col, a.n);
-            store_piece<T, VEC>(ou, dup + a.row * ld.x + a.col, a.n);
-            if (ACT) store_piece<T, VEC>(oa, act + a.row * shape.h + a.col, a.n);
-        }
-    }
+    store_piece<T, N, VEC>(og, dgate + a.row * ld.x + a.col, a.n);
+    store_piece<T, N, VEC>(ou, dup + a.row * ld.x + a.col, a.n);
+    if (ACT) store_piece<T, N, VEC>(oa, act + a.row * shape.h + a.col, a.n);
 }
 
 // ---- routing weights' gradient: d_gates[t, s] = <expert output s of token t (kept in 8 bits), grad_out[t]> ------------------
@@ -216,25 +193,26 @@ __global__ void __launch_bounds__(256)
     combine_bwd_gates_mx8_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                  const typename T::storage_t* __restrict__ grad_out,
                                  typename T::storage_t* __restrict__ d_gates, int64_t tokens, int k, int64_t H) {
+    constexpr int N = kMxPiece<T>;
     const int64_t t = (int64_t)blockIdx.x * 4 + threadIdx.x / CK_WAVE;
     if (t >= tokens) return;
     const int lane = lane_id();
     const int64_t blocks = (H + kMxBlock - 1) / kMxBlock;
-    const int64_t pieces = (H + kMxPiece - 1) / kMxPiece;
+    const int64_t pieces = (H + N - 1) / N;
     const typename T::storage_t* dy = grad_out + t * H;
     for (int s = 0; s < k; ++s) {
         const int64_t row = t * k + s;
         float acc = 0.f;
         for (int64_t p = lane; p < pieces; p += CK_WAVE) {
-            const int64_t left = H - p * kMxPiece;
-            const int n = left >= kMxPiece ? kMxPiece : (int)left;
-            const MxCodes c = load_codes<VEC>(codes + row * H + p * kMxPiece, n);
-            const float step = mx_step(scales[row * blocks + p / kMxQuad]);
-            const Piece<T> b = load_piece<T, VEC, false>(dy + p * kMxPiece, n);  // (re-read per slot: stays in the caches)
-            float v[kMxPiece];
+            const int64_t left = H - p * N;
+            const int n = left >= N ? N : (int)left;
+            const MxCodes<N> c = load_codes<N, VEC>(codes + row * H + p * N, n);
+            const float step = mx_step(scales[row * blocks + p / (kMxBlock / N)]);
+            const Piece<T, N> b = load_piece<T, N, VEC, false>(dy + p * N, n);  // (re-read per slot: stays in the caches)
+            float v[N];
             mx_decode(c, step, v);
 #pragma unroll
-            for (int j = 0; j < kMxPiece; ++j)
+            for (int j = 0; j < N; ++j)
                 if (VEC || j < n) acc += v[j] * b.up(j);
         }
         acc = wave_sum(acc);
@@ -245,11 +223,12 @@ __global__ void __launch_bounds__(256)
 }  // namespace ck
 
 // ---- host side ---------------------------------------------------------------------------------------------------------
+static int mx_piece(int dtype) { return dtype == CK_F32 ? 4 : 8; }
 static bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
 
 // kMxRows wherever every row starts on a whole packet, kMxFlat where the rows are one run besides
-static int mx_mode(int64_t h, bool aligned, bool dense) {
-    if (!aligned || h % ck::kMxPiece != 0) return ck::kMxAny;
+static int mx_mode(int64_t h, int piece, bool aligned, bool dense) {
+    if (!aligned || h % piece != 0) return ck::kMxAny;
     return dense && h % ck::kMxBlock == 0 ? ck::kMxFlat : ck::kMxRows;
 }
 
@@ -277,9 +256,9 @@ extern "C" int ck_mx8_quantize(const void* x, void* codes, void* scales, int64_t
     if (!x || !codes || !scales) return CK_ERR_NULL;
     if (!ck_aligned_elem(x, dtype)) return CK_ERR_ALIGN;
     ck::MxShape shape;
-    if (!ck::mx_shape(rows, H, &shape)) return CK_ERR_SHAPE;
+    if (!ck::mx_shape(rows, H, mx_piece(dtype), &shape)) return CK_ERR_SHAPE;
     hipStream_t s = (hipStream_t)stream;
-    const int mode = mx_mode(H, ck_aligned16(x) && aligned8(codes), true);
+    const int mode = mx_mode(H, mx_piece(dtype), ck_aligned16(x) && aligned8(codes), true);
     CK_DISPATCH_DTYPE(dtype, {
         typedef typename T::storage_t S;
         CK_MX_MODE(mode, {
@@ -298,9 +277,9 @@ extern "C" int ck_mx8_dequantize(const void* codes, const void* scales, const in
     if (!output || (source_rows > 0 && (!codes || !scales))) return CK_ERR_NULL;
     if (!ck_aligned_elem(output, dtype)) return CK_ERR_ALIGN;
     ck::MxShape shape;
-    if (!ck::mx_shape(rows, H, &shape)) return CK_ERR_SHAPE;
+    if (!ck::mx_shape(rows, H, mx_piece(dtype), &shape)) return CK_ERR_SHAPE;
     hipStream_t s = (hipStream_t)stream;
-    const int mode = mx_mode(H, ck_aligned16(output) && aligned8(codes), index == nullptr);
+    const int mode = mx_mode(H, mx_piece(dtype), ck_aligned16(output) && aligned8(codes), index == nullptr);
     CK_DISPATCH_DTYPE(dtype, {
         typedef typename T::storage_t S;
         if (index == nullptr) {
@@ -331,17 +310,17 @@ extern "C" int ck_swiglu_forward_mx8(const void* gate, const void* up, int64_t l
     if (!gate || !up || !output || !gate_codes || !up_codes || !gate_scales || !up_scales) return CK_ERR_NULL;
     if (!ck_aligned_elem(gate, dtype) || !ck_aligned_elem(up, dtype) || !ck_aligned_elem(output, dtype)) return CK_ERR_ALIGN;
     ck::MxShape shape;
-    if (!ck::mx_shape(rows, H, &shape)) return CK_ERR_SHAPE;
+    if (!ck::mx_shape(rows, H, mx_piece(dtype), &shape)) return CK_ERR_SHAPE;
     hipStream_t s = (hipStream_t)stream;
     const bool aligned = ck_aligned16(gate) && ck_aligned16(up) && ck_aligned16(output) && aligned8(gate_codes) &&
-                         aligned8(up_codes) && ldx % ck::kMxPiece == 0 && ldc % ck::kMxPiece == 0;
+                         aligned8(up_codes) && ldx % mx_piece(dtype) == 0 && ldc % mx_piece(dtype) == 0;
     const bool dense = ldx == H && ldc == H && lds == ck::mx_blocks(H);
-    const int mode = mx_mode(H, aligned, dense);
+    const int mode = mx_mode(H, mx_piece(dtype), aligned, dense);
     const ck::MxStrides ld = {ldx, ldc, lds};
     CK_DISPATCH_DTYPE(dtype, {
         typedef typename T::storage_t S;
         CK_MX_MODE(mode, {
-            hipLaunchKernelGGL((ck::swiglu_fwd_mx8_kernel<T, MODE>), mx_grid(shape, 2), dim3(ck::kMxThreads), 0, s,
+            hipLaunchKernelGGL((ck::swiglu_fwd_mx8_kernel<T, MODE>), mx_grid(shape, 1), dim3(ck::kMxThreads), 0, s,
                                (const S*)gate, (const S*)up, (S*)output, (int8_t*)gate_codes, (int8_t*)up_codes,
                                (uint8_t*)gate_scales, (uint8_t*)up_scales, ld, shape);
         });
@@ -361,24 +340,24 @@ extern "C" int ck_swiglu_backward_mx8(const void* gate_codes, const void* up_cod
         !ck_aligned_elem(activation, dtype))
         return CK_ERR_ALIGN;
     ck::MxShape shape;
-    if (!ck::mx_shape(rows, H, &shape)) return CK_ERR_SHAPE;
+    if (!ck::mx_shape(rows, H, mx_piece(dtype), &shape)) return CK_ERR_SHAPE;
     hipStream_t s = (hipStream_t)stream;
     const bool aligned = ck_aligned16(output_grad) && ck_aligned16(gate_grad) && ck_aligned16(up_grad) &&
                          ck_aligned16(activation) && aligned8(gate_codes) && aligned8(up_codes) &&
-                         ldx % ck::kMxPiece == 0 && ldc % ck::kMxPiece == 0;
+                         ldx % mx_piece(dtype) == 0 && ldc % mx_piece(dtype) == 0;
     const bool dense = ldx == H && ldc == H && lds == ck::mx_blocks(H);
-    const int mode = mx_mode(H, aligned, dense);
+    const int mode = mx_mode(H, mx_piece(dtype), aligned, dense);
     const ck::MxStrides ld = {ldx, ldc, lds};
     CK_DISPATCH_DTYPE(dtype, {
         typedef typename T::storage_t S;
         CK_MX_MODE(mode, {
             if (activation)
-                hipLaunchKernelGGL((ck::swiglu_bwd_mx8_kernel<T, MODE, true>), mx_grid(shape, 2), dim3(ck::kMxThreads), 0, s,
+                hipLaunchKernelGGL((ck::swiglu_bwd_mx8_kernel<T, MODE, true>), mx_grid(shape, 1), dim3(ck::kMxThreads), 0, s,
                                    (const int8_t*)gate_codes, (const int8_t*)up_codes, (const uint8_t*)gate_scales,
                                    (const uint8_t*)up_scales, (const S*)output_grad, (S*)gate_grad, (S*)up_grad,
                                    (S*)activation, ld, shape);
             else
-                hipLaunchKernelGGL((ck::swiglu_bwd_mx8_kernel<T, MODE, false>), mx_grid(shape, 2), dim3(ck::kMxThreads), 0,
+                hipLaunchKernelGGL((ck::swiglu_bwd_mx8_kernel<T, MODE, false>), mx_grid(shape, 1), dim3(ck::kMxThreads), 0,
                                    s, (const int8_t*)gate_codes, (const int8_t*)up_codes, (const uint8_t*)gate_scales,
                                    (const uint8_t*)up_scales, (const S*)output_grad, (S*)gate_grad, (S*)up_grad,
                                    (S*)nullptr, ld, shape);
@@ -397,7 +376,7 @@ extern "C" int ck_moe_combine_backward_gates_mx8(const void* codes, const void* 
     const int64_t grid = ck_ceil_div(tokens, 4);
     if (grid > 0x7fffffff) return CK_ERR_SHAPE;
     hipStream_t s = (hipStream_t)stream;
-    const bool vec = aligned8(codes) && ck_aligned16(grad_out) && H % ck::kMxPiece == 0;
+    const bool vec = aligned8(codes) && ck_aligned16(grad_out) && H % mx_piece(dtype) == 0;
     CK_DISPATCH_DTYPE(dtype, {
         typedef typename T::storage_t S;
         if (vec)

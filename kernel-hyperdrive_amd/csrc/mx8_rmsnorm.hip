@@ -3,54 +3,78 @@
 //             (and s itself with a residual)
 //   backward: with s^ the kept row:  dx = r (dy w - s^ r^2 mean(dy w s^)) (+ the sum's own gradient),  dw = sum dy s^ r
 // The row (forward: as read; backward: codes and dy) stays in the registers of a team of TPR lanes, so it is read once;
-// row sums are wave64 shuffles, wider teams meet through LDS.  A lane holds pieces of eight elements, lane t the pieces
-// t, t + TPR, ..: the four lanes of a quad hold one block.  Backward: every team walks rows and keeps its share of dw in
+// row sums are wave64 shuffles, wider teams meet through LDS.  Lane t holds the 16-byte pieces t, t + TPR, ..: neighbouring
+// lanes hold a block.  Backward: every team walks rows and keeps its share of dw in
 // fp32 registers; a workgroup writes one partial row, a second launch adds the partial rows up.  No atomics.
 #include "ck_mx8.h"
 
 namespace ck {
 
-constexpr int kMxMaxPieces = 8;  // of a lane
 
+// The backward's launch: workgroups a compute unit holds, and rows a team has in flight, by element size and team width.
+// Measured at 16384 x 4096 bf16 (and 8192 x 4096 fp32): three workgroups with one row in flight 69.1 us, two rows 69.4, three
+// rows 69.0 but 120 registers; four workgroups 71-79 (more partial rows of dw to write and add); fp32 with two
+// workgroups and two rows 57.8, three and one 58.7.
+constexpr int mx_bwd_residency(int bytes, int tpr) {
+    const int most = bytes == 4 ? 2 : 3;
+    return tpr == 1024 ? 1 : (tpr == 512 ? (most + 1) / 2 : most);
+}
+constexpr int mx_bwd_depth(int bytes, int tpr) { return bytes == 4 && tpr < 1024 ? 2 : 1; }
+
+// sum over the TPR lanes of a team, in all of them.  Teams wider than a wave meet at one barrier (every thread of the
+// workgroup comes here); `red` holds a float per wave, and two uses in a row take different ones.
 template <int TPR>
 __device__ __forceinline__ float mx_team_sum(float v, float* red) {
     v = wave_sum(v);
     if (TPR > CK_WAVE) {
-        __syncthreads();  // the previous use of `red`
-        if (lane_id() == 0) red[threadIdx.x / CK_WAVE] = v;
+        const int wave = threadIdx.x / CK_WAVE;
+        if (lane_id() == 0) red[wave] = v;
         __syncthreads();
+        const int first = wave / (TPR / CK_WAVE) * (TPR / CK_WAVE);
         v = 0.f;
 #pragma unroll
-        for (int w = 0; w < TPR / CK_WAVE; ++w) v += red[w];
+        for (int w = 0; w < TPR / CK_WAVE; ++w) v += red[first + w];
     }
     return v;
 }
 
-__device__ __forceinline__ int mx_piece_size(int H, int p) {
-    const int left = H - p * kMxPiece;
-    return left >= kMxPiece ? kMxPiece : (left > 0 ? left : 0);
+// Makes the compiler forget what it knows about a packed register set: values widened from it before this point are not
+// kept alive in place of the packed form.
+template <typename P>
+__device__ __forceinline__ void forget(P& p) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&p);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(P) / 4); ++i) asm volatile("" : "+v"(w[i]));
 }
 
-// one row per team; NP pieces a lane at most
-template <typename T, int TPR, int NP, bool RES, bool VEC>
+// elements of piece p that exist
+template <int N>
+__device__ __forceinline__ int mx_piece_size(int H, int p) {
+    const int left = H - p * N;
+    return left >= N ? N : (left > 0 ? left : 0);
+}
+
+// one row per team; UNITS units of eight elements a lane at most
+template <typename T, int TPR, int UNITS, bool RES, bool VEC>
 __global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
     rmsnorm_fwd_mx8_kernel(const typename T::storage_t* __restrict__ x, const typename T::storage_t* __restrict__ res,
                            const typename T::storage_t* __restrict__ w, typename T::storage_t* __restrict__ y,
                            typename T::storage_t* __restrict__ res_out, int8_t* __restrict__ codes,
                            uint8_t* __restrict__ scales, float* __restrict__ rstd_out, int64_t B, int H, float eps) {
+    constexpr int N = kMxPiece<T>, NP = UNITS * 8 / N;
     __shared__ float red[16];
     const int t = threadIdx.x % TPR;
     const int64_t row = (int64_t)blockIdx.x * (blockDim.x / TPR) + threadIdx.x / TPR;
-    if (row >= B) return;  // (a whole team; with TPR > 64 the workgroup is one team)
+    const bool live = row < B;
     const int blocks = (H + kMxBlock - 1) / kMxBlock;
     const typename T::storage_t* xr = x + row * H;
-    Piece<T> v[NP], r[RES ? NP : 1];
+    Piece<T, N> v[NP], r[RES ? NP : 1];
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-        const int p = t + i * TPR, n = mx_piece_size(H, p);
-        if (n > 0) {
-            v[i] = load_piece<T, VEC>(xr + p * kMxPiece, n);
-            if (RES) r[RES ? i : 0] = load_piece<T, VEC>(res + row * H + p * kMxPiece, n);
+        const int p = t + i * TPR, n = mx_piece_size<N>(H, p);
+        if (live && n > 0) {
+            v[i] = load_piece<T, N, VEC>(xr + p * N, n);
+            if (RES) r[RES ? i : 0] = load_piece<T, N, VEC>(res + row * H + p * N, n);
         } else {
             v[i].clear();
             if (RES) r[RES ? i : 0].clear();
@@ -60,7 +84,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
 #pragma unroll
-        for (int j = 0; j < kMxPiece; ++j) {
+        for (int j = 0; j < N; ++j) {
             // the sum is rounded to the storage type first: that value is the new residual and the row normalised
             if (RES) v[i].put(j, v[i].up(j) + r[RES ? i : 0].up(j));
             const float f = v[i].up(j);
@@ -69,155 +93,194 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
     }
     ss = mx_team_sum<TPR>(ss, red);
     const float rstd = rsqrtf(ss / (float)H + eps);
-    if (t == 0) rstd_out[row] = rstd;
+    if (live && t == 0) rstd_out[row] = rstd;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-        const int p = t + i * TPR, n = mx_piece_size(H, p);
-        float f[kMxPiece];
+        const int p = t + i * TPR, n = mx_piece_size<N>(H, p);
+        float f[N];
 #pragma unroll
-        for (int j = 0; j < kMxPiece; ++j) f[j] = v[i].up(j);
+        for (int j = 0; j < N; ++j) f[j] = v[i].up(j);
         uint32_t scale;
-        const MxCodes c = mx_encode(f, scale);
-        if (n > 0) {
-            Piece<T> o;
+        const MxCodes<N> c = mx_encode(f, scale);
+        if (live && n > 0) {
+            Piece<T, N> o;
             if (w != nullptr) {
-                const Piece<T> wv = load_piece<T, VEC, false>(w + p * kMxPiece, n);
+                const Piece<T, N> wv = load_piece<T, N, VEC, false>(w + p * N, n);
 #pragma unroll
-                for (int j = 0; j < kMxPiece; ++j) o.put(j, f[j] * rstd * wv.up(j));
+                for (int j = 0; j < N; ++j) o.put(j, f[j] * rstd * wv.up(j));
             } else {
 #pragma unroll
-                for (int j = 0; j < kMxPiece; ++j) o.put(j, f[j] * rstd);
+                for (int j = 0; j < N; ++j) o.put(j, f[j] * rstd);
             }
-            store_piece<T, VEC>(o, y + row * H + p * kMxPiece, n);
-            if (RES) store_piece<T, VEC>(v[i], res_out + row * H + p * kMxPiece, n);
-            store_codes<VEC>(c, codes + row * H + p * kMxPiece, n);
-            if (t % kMxQuad == 0) scales[row * blocks + p / kMxQuad] = (uint8_t)scale;
+            store_piece<T, N, VEC>(o, y + row * H + p * N, n);
+            if (RES) store_piece<T, N, VEC>(v[i], res_out + row * H + p * N, n);
+            store_codes<N, VEC>(c, codes + row * H + p * N, n);
+            if (t % kMxLanes<T> == 0) scales[row * blocks + p / kMxLanes<T>] = (uint8_t)scale;
         }
     }
 }
 
-// Teams walk rows.  dy and the weight are kept in registers with the codes, except by the 1024-lane team, whose lanes have
-// 128 registers: it reads dy and the weight twice, the second time from the cache.
-template <typename T, int TPR, int NP, bool HAS_W, bool VEC>
-__global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
+// Rows are dealt round-robin to the teams; a team has the next row in flight while it works on one.
+// With q the codes and e the step of a block:  dx = r (dy w) - (r^3 mean(dy w s^) e) q,  dw += (dy e r) q  - the steps are
+// folded into factors of a piece, so the kept row costs one conversion an element and no multiplication of its own.
+template <typename T, int TPR, int UNITS, bool HAS_W, bool DSUM, bool VEC>
+__global__ void __launch_bounds__(TPR > 256 ? TPR : 256, mx_bwd_residency(sizeof(typename T::storage_t), TPR))
     rmsnorm_bwd_mx8_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                            const typename T::storage_t* __restrict__ w, const typename T::storage_t* __restrict__ dy,
                            const float* __restrict__ rstd_in, const typename T::storage_t* __restrict__ dsum,
                            typename T::storage_t* __restrict__ dx, float* __restrict__ dw_partial, int64_t B, int H) {
-    constexpr bool LEAN = TPR == 1024;
+    constexpr int N = kMxPiece<T>, NP = UNITS * 8 / N;
+    constexpr int THREADS = TPR > 256 ? TPR : 256, TEAMS = THREADS / TPR;
+    // A lane of the 1024-lane team has 128 registers.  Where its sums of dw and a row leave no room beside each other, nothing
+    // of the row is kept: it is read twice, the second time from the cache.
+    constexpr bool LEAN = TPR == 1024 && UNITS * sizeof(typename T::storage_t) > 8;
     constexpr int KEEP = LEAN ? 1 : NP;
-    __shared__ float red[16];
-    const int teams_per_block = blockDim.x / TPR;
-    const int t = threadIdx.x % TPR;
-    const int64_t team = (int64_t)blockIdx.x * teams_per_block + threadIdx.x / TPR;
-    const int64_t num_teams = (int64_t)gridDim.x * teams_per_block;
+    __shared__ float red[2][THREADS / CK_WAVE];
+    const int t = threadIdx.x % TPR, team = threadIdx.x / TPR;
     const int blocks = (H + kMxBlock - 1) / kMxBlock;
     const float inv_h = 1.f / (float)H;
 
-    Piece<T> wv[HAS_W ? KEEP : 1];
-    float dw[HAS_W ? NP : 1][kMxPiece];
+    struct Row {
+        MxCodes<N> c[KEEP];
+        uint32_t scale[KEEP];
+        Piece<T, N> g[KEEP], s[DSUM ? KEEP : 1];
+        float rstd;
+    };
+    // piece i of a row into place k of a Row
+    auto fetch_piece = [&](int64_t row, int i, int k, Row& r) __attribute__((always_inline)) {
+        const int p = t + i * TPR, n = mx_piece_size<N>(H, p);
+        r.c[k] = MxCodes<N>{};
+        r.scale[k] = 7;
+        r.g[k].clear();
+        if (row < B && n > 0) {
+            r.c[k] = load_codes<N, VEC>(codes + row * H + p * N, n);
+            r.scale[k] = scales[row * blocks + p / kMxLanes<T>];
+            r.g[k] = load_piece<T, N, VEC, !LEAN>(dy + row * H + p * N, n);
+            if (DSUM) r.s[DSUM ? k : 0] = load_piece<T, N, VEC, !LEAN>(dsum + row * H + p * N, n);
+        }
+    };
+    auto fetch = [&](int64_t row, Row& r) __attribute__((always_inline)) {
+        r.rstd = row < B ? rstd_in[row] : 0.f;
+        if (!LEAN) {
+#pragma unroll
+            for (int i = 0; i < NP; ++i) fetch_piece(row, i, LEAN ? 0 : i, r);
+        }
+    };
+
+    Piece<T, N> wv[HAS_W ? KEEP : 1];
+    float dw[HAS_W ? NP : 1][N];
     if (HAS_W) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-            const int p = t + i * TPR, n = mx_piece_size(H, p);
+            const int p = t + i * TPR, n = mx_piece_size<N>(H, p);
             if (!LEAN) {
-                if (n > 0) wv[LEAN ? 0 : i] = load_piece<T, VEC, false>(w + p * kMxPiece, n);
-                else wv[LEAN ? 0 : i].clear();
+                wv[LEAN ? 0 : i].clear();
+                if (n > 0) wv[LEAN ? 0 : i] = load_piece<T, N, VEC, false>(w + p * N, n);
             }
 #pragma unroll
-            for (int j = 0; j < kMxPiece; ++j) dw[i][j] = 0.f;
+            for (int j = 0; j < N; ++j) dw[i][j] = 0.f;
         }
     }
-    for (int64_t row = team; row < B; row += num_teams) {
-        const typename T::storage_t* gr = dy + row * H;
-        const float rstd = rstd_in[row];
-        MxCodes c[NP];
-        uint32_t scale[NP];
-        Piece<T> g[KEEP];
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            const int p = t + i * TPR, n = mx_piece_size(H, p);
-            c[i].w[0] = c[i].w[1] = 0;
-            scale[i] = 7;
-            if (!LEAN) g[LEAN ? 0 : i].clear();
-            if (n > 0) {
-                c[i] = load_codes<VEC>(codes + row * H + p * kMxPiece, n);
-                scale[i] = scales[row * blocks + p / kMxQuad];
-                if (!LEAN) g[LEAN ? 0 : i] = load_piece<T, VEC>(gr + p * kMxPiece, n);
-            }
-        }
+    auto work = [&](int64_t row, Row& cur, int turn) __attribute__((always_inline)) {
+        const bool live = row < B;
         float dot = 0.f;
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-            const int p = t + i * TPR, n = mx_piece_size(H, p);
-            if (n > 0) {
-                float f[kMxPiece];
-                mx_decode(c[i], mx_step(scale[i]), f);
-                const Piece<T> gp = LEAN ? load_piece<T, VEC, false>(gr + p * kMxPiece, n) : g[LEAN ? 0 : i];
-                Piece<T> wp;
-                if (HAS_W) wp = LEAN ? load_piece<T, VEC, false>(w + p * kMxPiece, n) : wv[LEAN ? 0 : i];
+            const int p = t + i * TPR, n = mx_piece_size<N>(H, p), at = LEAN ? 0 : i;
+            if (live && n > 0) {
+                if (LEAN) fetch_piece(row, i, 0, cur);
+                Piece<T, N> wp;
+                if (HAS_W) wp = LEAN ? load_piece<T, N, VEC, false>(w + p * N, n) : wv[HAS_W ? at : 0];
+                float part = 0.f;
 #pragma unroll
-                for (int j = 0; j < kMxPiece; ++j) {
-                    if (!VEC && j >= n) continue;  // (a block that stands for NaNs must not reach past the row)
-                    dot += gp.up(j) * (HAS_W ? wp.up(j) : 1.f) * f[j];
-                }
+                for (int j = 0; j < N; ++j)
+                    part += (HAS_W ? cur.g[at].up(j) * wp.up(j) : cur.g[at].up(j)) * mx_code(cur.c[at], j);
+                dot += part * mx_step(cur.scale[at]);
+            }
+            __builtin_amdgcn_sched_barrier(0);  // one piece at a time: widened values do not pile up in registers
+        }
+        if (!LEAN) {
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const int at = LEAN ? 0 : i;
+                forget(cur.g[at]);
+                forget(cur.c[at]);
+                if (HAS_W) forget(wv[HAS_W ? at : 0]);
             }
         }
-        dot = mx_team_sum<TPR>(dot, red);
-        const float k = rstd * rstd * rstd * inv_h * dot;
+        dot = mx_team_sum<TPR>(dot, red[turn]);
+        const float rstd = cur.rstd, k = rstd * rstd * rstd * inv_h * dot;
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-            const int p = t + i * TPR, n = mx_piece_size(H, p);
-            if (n > 0) {
-                float f[kMxPiece];
-                mx_decode(c[i], mx_step(scale[i]), f);
-                const Piece<T> gp = LEAN ? load_piece<T, VEC, false>(gr + p * kMxPiece, n) : g[LEAN ? 0 : i];
-                Piece<T> wp, sp, o;
-                if (HAS_W) wp = LEAN ? load_piece<T, VEC, false>(w + p * kMxPiece, n) : wv[LEAN ? 0 : i];
-                if (dsum != nullptr) sp = load_piece<T, VEC>(dsum + row * H + p * kMxPiece, n);
+            const int p = t + i * TPR, n = mx_piece_size<N>(H, p), at = LEAN ? 0 : i;
+            if (live && n > 0) {
+                if (LEAN) fetch_piece(row, i, 0, cur);
+                Piece<T, N> wp, o;
+                if (HAS_W) wp = LEAN ? load_piece<T, N, VEC, false>(w + p * N, n) : wv[HAS_W ? at : 0];
+                const float e = mx_step(cur.scale[at]), ke = k * e, er = e * rstd;
 #pragma unroll
-                for (int j = 0; j < kMxPiece; ++j) {
-                    const float d = gp.up(j);
-                    if (HAS_W && (VEC || j < n)) dw[HAS_W ? i : 0][j] += d * (f[j] * rstd);
-                    float out = rstd * (HAS_W ? d * wp.up(j) : d) - k * f[j];
-                    if (dsum != nullptr) out += sp.up(j);
+                for (int j = 0; j < N; ++j) {
+                    const float d = cur.g[at].up(j), q = mx_code(cur.c[at], j);
+                    if (HAS_W) dw[HAS_W ? i : 0][j] += d * er * q;
+                    float out = rstd * (HAS_W ? d * wp.up(j) : d) - ke * q;
+                    if (DSUM) out += cur.s[DSUM ? at : 0].up(j);
                     o.put(j, out);
                 }
-                store_piece<T, VEC>(o, dx + row * H + p * kMxPiece, n);
+                store_piece<T, N, VEC>(o, dx + row * H + p * N, n);
             }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    const int64_t step = (int64_t)gridDim.x * TEAMS;
+    int64_t first = (int64_t)blockIdx.x * TEAMS, row = first + team;
+    // rows in flight while one is worked on; a row's place is filled again as soon as it is done with
+    constexpr int DEPTH = LEAN ? 1 : mx_bwd_depth(sizeof(typename T::storage_t), TPR);
+    Row buf[DEPTH];
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) fetch(row + d * step, buf[d]);
+    int turn = 0;
+    while (first < B) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            if (first < B) {
+                work(row, buf[d], turn);
+                turn ^= 1;
+                fetch(row + DEPTH * step, buf[d]);
+            }
+            first += step;
+            row += step;
         }
     }
     if (HAS_W) {
-        // one partial row per workgroup; the four teams of a 256-lane workgroup are added up in LDS, in their order
+        // one partial row per workgroup; its teams are added up in LDS, in their order
         const int padded = blocks * kMxBlock;
-        constexpr int kTeams = TPR == 64 ? 4 : 1;
-        constexpr int kCols = TPR == 64 ? 64 * NP * kMxPiece : 4;
-        __shared__ float comb[kTeams * kCols];
-        float* out = kTeams > 1 ? comb + (threadIdx.x / TPR) * kCols : dw_partial + (int64_t)blockIdx.x * padded;
+        constexpr int kCols = TEAMS > 1 ? TPR * NP * N : 4;
+        __shared__ float comb[TEAMS * kCols];
+        float* out = TEAMS > 1 ? comb + team * kCols : dw_partial + (int64_t)blockIdx.x * padded;
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
             const int p = t + i * TPR;
-            if (p < blocks * kMxQuad) {
+            if (p < blocks * kMxLanes<T>) {
 #pragma unroll
-                for (int j = 0; j < kMxPiece; j += 4)
-                    *reinterpret_cast<float4*>(out + p * kMxPiece + j) = make_float4(
+                for (int j = 0; j < N; j += 4)
+                    *reinterpret_cast<float4*>(out + p * N + j) = make_float4(
                         dw[HAS_W ? i : 0][j], dw[HAS_W ? i : 0][j + 1], dw[HAS_W ? i : 0][j + 2], dw[HAS_W ? i : 0][j + 3]);
             }
         }
-        if (kTeams > 1) {
+        if (TEAMS > 1) {
             __syncthreads();
-            float* row = dw_partial + (int64_t)blockIdx.x * padded;
-            for (int col = threadIdx.x * 4; col < padded; col += blockDim.x * 4) {
+            float* sum = dw_partial + (int64_t)blockIdx.x * padded;
+            for (int col = threadIdx.x * 4; col < padded; col += THREADS * 4) {
                 float4 a = *reinterpret_cast<const float4*>(comb + col);
 #pragma unroll
-                for (int m = 1; m < kTeams; ++m) {
+                for (int m = 1; m < TEAMS; ++m) {
                     const float4 b = *reinterpret_cast<const float4*>(comb + m * kCols + col);
                     a.x += b.x;
                     a.y += b.y;
                     a.z += b.z;
                     a.w += b.w;
                 }
-                *reinterpret_cast<float4*>(row + col) = a;
+                *reinterpret_cast<float4*>(sum + col) = a;
             }
         }
     }
@@ -273,15 +336,27 @@ namespace {
 
 constexpr int64_t kMxMaxRow = 65536;
 
-// lanes per row, and pieces per lane of the narrowest instantiation that holds it
+// units of eight elements in a row
+int64_t mx_row_units(int64_t H) { return ck::mx_blocks(H) * 4; }
+
+// Lanes per row, both ways: two units a lane (more only beyond 16384 elements).  Few registers keep many waves resident:
+// forward 59.5 us at 16384 x 4096 bf16, against 59.8 with four units a lane and 66.1 with a wave per row.
 int mx_tpr(int64_t H) {
-    const int64_t pieces = ck::mx_blocks(H) * ck::kMxQuad;
-    return pieces <= 64 * ck::kMxMaxPieces ? 64 : (pieces <= 256 * ck::kMxMaxPieces ? 256 : 1024);
+    const int64_t units = mx_row_units(H);
+    for (int tpr : {64, 128, 256, 512})
+        if (units <= (int64_t)tpr * 2) return tpr;
+    return 1024;
 }
-int mx_pieces(int64_t H, int tpr) {
-    const int64_t pieces = ck::mx_blocks(H) * ck::kMxQuad;
-    for (int np : {1, 2, 4})
-        if (pieces <= (int64_t)np * tpr) return np;
+// the team the backward's launch takes: those of 128 and 512 lanes only for aligned rows
+int mx_bwd_tpr(int64_t H, bool vec) {
+    const int tpr = mx_tpr(H);
+    return vec ? tpr : (tpr == 128 ? 256 : (tpr == 512 ? 1024 : tpr));
+}
+// the fewest units a lane has to hold, of those compiled
+int mx_units(int64_t H, int tpr) {
+    const int64_t units = mx_row_units(H);
+    for (int n : {1, 2, 4})
+        if (units <= (int64_t)n * tpr) return n;
     return 8;
 }
 
@@ -298,10 +373,10 @@ int mx_cu_count() {
 }
 
 // workgroups of the backward: each writes one partial row of dw
-int mx_bwd_blocks(int64_t B, int64_t H) {
-    const int tpr = mx_tpr(H);
-    const int64_t need = ck_ceil_div(B, tpr == 64 ? 4 : 1);
-    const int64_t most = (int64_t)mx_cu_count() * (tpr == 64 && mx_pieces(H, tpr) <= 4 ? 2 : 1);
+int mx_bwd_blocks(int64_t B, int64_t H, int dtype, bool vec) {
+    const int tpr = mx_bwd_tpr(H, vec);
+    const int64_t need = ck_ceil_div(B, tpr < 256 ? 256 / tpr : 1);
+    const int64_t most = (int64_t)mx_cu_count() * ck::mx_bwd_residency(dtype == CK_F32 ? 4 : 2, tpr);
     return (int)(need < most ? need : most);
 }
 
@@ -313,32 +388,26 @@ struct MxFwd {
     int H;
     float eps;
 };
-template <typename T, int TPR, int NP, bool RES, bool VEC>
+template <typename T, int TPR, int UNITS, bool RES, bool VEC>
 void mx_launch_fwd(hipStream_t s, const MxFwd& a) {
     typedef typename T::storage_t S;
     constexpr int block = TPR > 256 ? TPR : 256;
-    hipLaunchKernelGGL((ck::rmsnorm_fwd_mx8_kernel<T, TPR, NP, RES, VEC>), dim3((unsigned)ck_ceil_div(a.B, block / TPR)),
+    hipLaunchKernelGGL((ck::rmsnorm_fwd_mx8_kernel<T, TPR, UNITS, RES, VEC>), dim3((unsigned)ck_ceil_div(a.B, block / TPR)),
                        dim3(block), 0, s, (const S*)a.x, (const S*)a.res, (const S*)a.w, (S*)a.y, (S*)a.res_out,
                        (int8_t*)a.codes, (uint8_t*)a.scales, a.rstd, a.B, a.H, a.eps);
 }
-template <typename T, bool RES>
-void mx_dispatch_fwd(hipStream_t s, const MxFwd& a, bool vec) {
-    const int tpr = mx_tpr(a.H), np = mx_pieces(a.H, tpr);
-    if (!vec) {
-        if (tpr == 64) mx_launch_fwd<T, 64, 8, RES, false>(s, a);
-        else if (tpr == 256) mx_launch_fwd<T, 256, 8, RES, false>(s, a);
-        else mx_launch_fwd<T, 1024, 8, RES, false>(s, a);
-    } else if (tpr == 64) {
-        if (np == 1) mx_launch_fwd<T, 64, 1, RES, true>(s, a);
-        else if (np == 2) mx_launch_fwd<T, 64, 2, RES, true>(s, a);
-        else if (np == 4) mx_launch_fwd<T, 64, 4, RES, true>(s, a);
-        else mx_launch_fwd<T, 64, 8, RES, true>(s, a);
-    } else if (tpr == 256) {
-        if (np <= 4) mx_launch_fwd<T, 256, 4, RES, true>(s, a);
-        else mx_launch_fwd<T, 256, 8, RES, true>(s, a);
-    } else {
-        mx_launch_fwd<T, 1024, 8, RES, true>(s, a);
-    }
+// teams of 128 and 512 lanes only where alignment lets them be fast: rows read element by element take the next wider one
+template <typename T, bool RES, bool VEC>
+void mx_dispatch_fwd(hipStream_t s, const MxFwd& a) {
+    const int tpr = mx_tpr(a.H), units = mx_units(a.H, tpr);
+    if (VEC && tpr == 64 && units == 1) mx_launch_fwd<T, 64, VEC ? 1 : 2, RES, VEC>(s, a);
+    else if (tpr == 64) mx_launch_fwd<T, 64, 2, RES, VEC>(s, a);
+    else if (VEC && tpr == 128) mx_launch_fwd<T, VEC ? 128 : 256, 2, RES, VEC>(s, a);
+    else if (tpr <= 256) mx_launch_fwd<T, 256, 2, RES, VEC>(s, a);
+    else if (VEC && tpr == 512) mx_launch_fwd<T, VEC ? 512 : 1024, 2, RES, VEC>(s, a);
+    else if (units <= 2) mx_launch_fwd<T, 1024, 2, RES, VEC>(s, a);
+    else if (units == 4) mx_launch_fwd<T, 1024, 4, RES, VEC>(s, a);
+    else mx_launch_fwd<T, 1024, 8, RES, VEC>(s, a);
 }
 
 struct MxBwd {
@@ -346,34 +415,31 @@ struct MxBwd {
     const float* rstd;
     void *dx, *ws;
     int64_t B;
-    int H;
+    int H, blocks;
 };
-template <typename T, int TPR, int NP, bool W, bool VEC>
+template <typename T, int TPR, int UNITS, bool W, bool D, bool VEC>
 void mx_launch_bwd(hipStream_t s, const MxBwd& a) {
     typedef typename T::storage_t S;
-    constexpr int block = TPR > 256 ? TPR : 256;
-    hipLaunchKernelGGL((ck::rmsnorm_bwd_mx8_kernel<T, TPR, NP, W, VEC>), dim3((unsigned)mx_bwd_blocks(a.B, a.H)), dim3(block),
+    hipLaunchKernelGGL((ck::rmsnorm_bwd_mx8_kernel<T, TPR, UNITS, W, D, VEC>), dim3((unsigned)a.blocks), dim3(TPR > 256 ? TPR : 256),
                        0, s, (const int8_t*)a.codes, (const uint8_t*)a.scales, (const S*)a.w, (const S*)a.dy, a.rstd,
                        (const S*)a.dsum, (S*)a.dx, (float*)a.ws, a.B, a.H);
 }
-template <typename T, bool W>
-void mx_dispatch_bwd(hipStream_t s, const MxBwd& a, bool vec) {
-    const int tpr = mx_tpr(a.H), np = mx_pieces(a.H, tpr);
-    if (!vec) {
-        if (tpr == 64) mx_launch_bwd<T, 64, 8, W, false>(s, a);
-        else if (tpr == 256) mx_launch_bwd<T, 256, 8, W, false>(s, a);
-        else mx_launch_bwd<T, 1024, 8, W, false>(s, a);
-    } else if (tpr == 64) {
-        if (np == 1) mx_launch_bwd<T, 64, 1, W, true>(s, a);
-        else if (np == 2) mx_launch_bwd<T, 64, 2, W, true>(s, a);
-        else if (np == 4) mx_launch_bwd<T, 64, 4, W, true>(s, a);
-        else mx_launch_bwd<T, 64, 8, W, true>(s, a);
-    } else if (tpr == 256) {
-        if (np <= 4) mx_launch_bwd<T, 256, 4, W, true>(s, a);
-        else mx_launch_bwd<T, 256, 8, W, true>(s, a);
-    } else {
-        mx_launch_bwd<T, 1024, 8, W, true>(s, a);
-    }
+template <typename T, bool W, bool D, bool VEC>
+void mx_dispatch_bwd_as(hipStream_t s, const MxBwd& a) {
+    const int tpr = mx_bwd_tpr(a.H, VEC), units = mx_units(a.H, tpr);
+    if (VEC && tpr == 64 && units == 1) mx_launch_bwd<T, 64, VEC ? 1 : 2, W, D, VEC>(s, a);
+    else if (tpr == 64) mx_launch_bwd<T, 64, 2, W, D, VEC>(s, a);
+    else if (VEC && tpr == 128) mx_launch_bwd<T, VEC ? 128 : 256, 2, W, D, VEC>(s, a);
+    else if (tpr == 256) mx_launch_bwd<T, 256, 2, W, D, VEC>(s, a);
+    else if (VEC && tpr == 512) mx_launch_bwd<T, VEC ? 512 : 1024, 2, W, D, VEC>(s, a);
+    else if (units <= 2) mx_launch_bwd<T, 1024, 2, W, D, VEC>(s, a);
+    else if (units == 4) mx_launch_bwd<T, 1024, 4, W, D, VEC>(s, a);
+    else mx_launch_bwd<T, 1024, 8, W, D, VEC>(s, a);
+}
+template <typename T, bool W, bool VEC>
+void mx_dispatch_bwd(hipStream_t s, const MxBwd& a) {
+    if (a.dsum) mx_dispatch_bwd_as<T, W, true, VEC>(s, a);
+    else mx_dispatch_bwd_as<T, W, false, VEC>(s, a);
 }
 
 bool mx_rows_dtype(int dtype) { return dtype == CK_F32 || dtype == CK_F16 || dtype == CK_BF16; }
@@ -390,7 +456,7 @@ extern "C" int ck_rmsnorm_forward_mx8(const void* x, const void* residual, const
     if (B > 0x7fffffff) return CK_ERR_SHAPE;
     if (!x || !output || !codes || !scales || !rstd || (residual && !residual_out)) return CK_ERR_NULL;
     const void* ptrs[5] = {x, residual, weight, output, residual_out};
-    bool vec = H % ck::kMxPiece == 0 && mx_aligned8(codes);
+    bool vec = H % (dtype == CK_F32 ? 4 : 8) == 0 && mx_aligned8(codes);
     for (const void* p : ptrs) {
         if (!ck_aligned_elem(p, dtype)) return CK_ERR_ALIGN;
         vec = vec && ck_aligned16(p);
@@ -399,15 +465,19 @@ extern "C" int ck_rmsnorm_forward_mx8(const void* x, const void* residual, const
     const MxFwd a = {x, residual, weight, output, residual_out, codes, scales, rstd, B, (int)H, eps};
     hipStream_t s = (hipStream_t)stream;
     CK_DISPATCH_DTYPE(dtype, {
-        if (residual) mx_dispatch_fwd<T, true>(s, a, vec);
-        else mx_dispatch_fwd<T, false>(s, a, vec);
+        if (residual && vec) mx_dispatch_fwd<T, true, true>(s, a);
+        else if (residual) mx_dispatch_fwd<T, true, false>(s, a);
+        else if (vec) mx_dispatch_fwd<T, false, true>(s, a);
+        else mx_dispatch_fwd<T, false, false>(s, a);
     });
     return ck_launch_status();
 }
 
-extern "C" int64_t ck_rmsnorm_backward_mx8_workspace_size(int64_t B, int64_t H) {
+extern "C" int64_t ck_rmsnorm_backward_mx8_workspace_size(int64_t B, int64_t H, int dtype) {
     if (B <= 0 || H <= 0 || H > kMxMaxRow) return 0;
-    return (int64_t)mx_bwd_blocks(B, H) * ck::mx_blocks(H) * ck::kMxBlock * 4;
+    // (whichever way the operands turn out to be aligned)
+    const int a = mx_bwd_blocks(B, H, dtype, true), b = mx_bwd_blocks(B, H, dtype, false);
+    return (int64_t)(a > b ? a : b) * ck::mx_blocks(H) * ck::kMxBlock * 4;
 }
 
 extern "C" int ck_rmsnorm_backward_mx8(const void* codes, const void* scales, const void* weight, const void* output_grad,
@@ -425,20 +495,22 @@ extern "C" int ck_rmsnorm_backward_mx8(const void* codes, const void* scales, co
     if (B > 0) {
         if (!codes || !scales || !output_grad || !rstd || !x_grad) return CK_ERR_NULL;
         const void* ptrs[4] = {weight, output_grad, sum_grad, x_grad};
-        bool vec = H % ck::kMxPiece == 0 && mx_aligned8(codes);
+        bool vec = H % (dtype == CK_F32 ? 4 : 8) == 0 && mx_aligned8(codes);
         for (const void* p : ptrs) {
             if (!ck_aligned_elem(p, dtype)) return CK_ERR_ALIGN;
             vec = vec && ck_aligned16(p);
         }
         if (reinterpret_cast<uintptr_t>(rstd) & 3u) return CK_ERR_ALIGN;
         if (weight && (!workspace || !ck_aligned16(workspace) ||
-                       workspace_bytes < ck_rmsnorm_backward_mx8_workspace_size(B, H)))
+                       workspace_bytes < ck_rmsnorm_backward_mx8_workspace_size(B, H, dtype)))
             return CK_ERR_WORKSPACE;
-        parts = mx_bwd_blocks(B, H);
-        const MxBwd a = {codes, scales, weight, output_grad, sum_grad, rstd, x_grad, workspace, B, (int)H};
+        parts = mx_bwd_blocks(B, H, dtype, vec);
+        const MxBwd a = {codes, scales, weight, output_grad, sum_grad, rstd, x_grad, workspace, B, (int)H, parts};
         CK_DISPATCH_DTYPE(dtype, {
-            if (weight) mx_dispatch_bwd<T, true>(s, a, vec);
-            else mx_dispatch_bwd<T, false>(s, a, vec);
+            if (weight && vec) mx_dispatch_bwd<T, true, true>(s, a);
+            else if (weight) mx_dispatch_bwd<T, true, false>(s, a);
+            else if (vec) mx_dispatch_bwd<T, false, true>(s, a);
+            else mx_dispatch_bwd<T, false, false>(s, a);
         });
     }
     if (weight) {

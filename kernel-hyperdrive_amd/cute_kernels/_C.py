@@ -94,7 +94,7 @@ _SIGNATURES = {
     "ck_swiglu_forward_mx8": (_i32, [_p, _p, _i64, _p, _p, _p, _i64, _p, _p, _i64, _i64, _i64, _i32, _p]),
     "ck_swiglu_backward_mx8": (_i32, [_p, _p, _i64, _p, _p, _i64, _p, _p, _p, _i64, _p, _i64, _i64, _i32, _p]),
     "ck_rmsnorm_forward_mx8": (_i32, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _f32, _i32, _p]),
-    "ck_rmsnorm_backward_mx8_workspace_size": (_i64, [_i64, _i64]),
+    "ck_rmsnorm_backward_mx8_workspace_size": (_i64, [_i64, _i64, _i32]),
     "ck_rmsnorm_backward_mx8": (_i32, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i32, _p]),
     "ck_moe_combine_backward_gates_mx8": (_i32, [_p, _p, _p, _p, _i64, _i64, _i64, _i32, _p]),
 }
@@ -1090,13 +1090,13 @@ def rmsnorm_forward_mx8(x, residual, weight, output, residual_out, codes, scales
         )
 
 
-def rmsnorm_backward_mx8_workspace_size(B: int, H: int, device: torch.device) -> int:
+def rmsnorm_backward_mx8_workspace_size(B: int, H: int, dtype: torch.dtype, device: torch.device) -> int:
     """Depends on the compute units of the device that is current in the call."""
     lib = load_library()
     if device.type != "cuda" or device.index == torch._C._cuda_getDevice():
-        return lib.ck_rmsnorm_backward_mx8_workspace_size(B, H)
+        return lib.ck_rmsnorm_backward_mx8_workspace_size(B, H, dtype_code(dtype))
     with torch.cuda.device(device):
-        return lib.ck_rmsnorm_backward_mx8_workspace_size(B, H)
+        return lib.ck_rmsnorm_backward_mx8_workspace_size(B, H, dtype_code(dtype))
 
 
 def rmsnorm_backward_mx8(codes, scales, weight, output_grad, rstd, sum_grad, x_grad, weight_grad, workspace) -> None:

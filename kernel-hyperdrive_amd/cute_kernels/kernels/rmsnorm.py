@@ -266,7 +266,9 @@ def rmsnorm_backward_mx8_hip(
     workspace = None
     if weight is not None:
         # fp32 partial rows of the dweight sum; taken from torch's caching allocator
-        nbytes = _C.rmsnorm_backward_mx8_workspace_size(rmsnorm_denominator.numel(), weight.numel(), weight.device)
+        nbytes = _C.rmsnorm_backward_mx8_workspace_size(
+            rmsnorm_denominator.numel(), weight.numel(), weight.dtype, weight.device
+        )
         workspace = torch.empty(max(nbytes, 16), device=weight.device, dtype=torch.uint8)
     _C.rmsnorm_backward_mx8(
         codes, scales, weight, output_grad, rmsnorm_denominator, sum_grad, x_grad, weight_grad, workspace

@@ -312,12 +312,14 @@ inline int emu_readfirstlane(int v) {
     return emu::wave_instruction(v, [](auto lane) { return lane(0); });
 }
 #define __builtin_amdgcn_readfirstlane(v) emu_readfirstlane(v)
-// v_mov_b32 with a quad_perm control (the only DPP form the kernels use): lane l reads lane 4 (l / 4) + (ctrl >> 2 (l % 4)) % 4
-inline int emu_quad_perm(int v, int ctrl) {
+// v_mov_b32 with the DPP controls the kernels use - quad_perm (0 .. 0xFF): lane l reads lane 4 (l / 4) + (ctrl >> 2 (l % 4)) % 4;
+// row_half_mirror (0x141): lane l reads lane 8 (l / 8) + 7 - l % 8
+inline int emu_mov_dpp(int v, int ctrl) {
     const int me = __lane_id();
-    return emu::wave_instruction(v, [me, ctrl](auto lane) { return lane(me / 4 * 4 + ((ctrl >> (2 * (me % 4))) & 3)); });
+    const int from = ctrl == 0x141 ? me / 8 * 8 + 7 - me % 8 : me / 4 * 4 + ((ctrl >> (2 * (me % 4))) & 3);
+    return emu::wave_instruction(v, [from](auto lane) { return lane(from); });
 }
-#define __builtin_amdgcn_mov_dpp(v, ctrl, row_mask, bank_mask, bound_ctrl) emu_quad_perm(v, ctrl)
+#define __builtin_amdgcn_mov_dpp(v, ctrl, row_mask, bank_mask, bound_ctrl) emu_mov_dpp(v, ctrl)
 #define __builtin_amdgcn_s_barrier() emu::sync(emu::g_block)
 // The lanes of a wavefront run in lock-step on the hardware; here they run freely between the instructions that make
 // them meet.  Where a kernel lets lanes of one wave talk through memory and relies on the lock-step, it says so with a
