@@ -991,58 +991,76 @@ def mx8_dequantize(codes, scales, output, index=None, fan: int = 1) -> None:
         )
 
 
-def swiglu_forward_mx8(gate, up, output, codes, scales) -> None:
-    """Two dense tensors of one shape; codes [2, ...] and scales: gate's, then up's."""
+# What an operator keeps for its backward is one int8 buffer: the codes of all its rows, then their scale bytes, then (RMSNorm)
+# 1 / rms per row in fp32, each part from a multiple of 16 on.
+def mx8_kept_offsets(rows: int, H: int, with_rstd: bool) -> tuple[int, int, int]:
+    """(offset of the scale bytes, offset of 1 / rms, bytes in all)"""
+    scales = rows * H + 15 & -16
+    end = scales + rows * -(-H // MX8_BLOCK)
+    if not with_rstd:
+        return scales, end, end
+    rstd = end + 15 & -16
+    return scales, rstd, rstd + 4 * rows
+
+
+def _kept_parts(what: str, kept, rows: int, H: int, with_rstd: bool) -> tuple[int, int]:
+    scales, rstd, total = mx8_kept_offsets(rows, H, with_rstd)
+    if kept.dtype != torch.int8 or kept.numel() != total or not kept.is_contiguous():
+        raise ValueError(f"{what}: the kept form is {total} dense int8, got {kept.numel()} {kept.dtype}")
+    return scales, rstd
+
+
+def swiglu_forward_mx8(gate, up, output, kept) -> None:
+    """Two dense tensors of one shape; kept: the rows of gate, then those of up."""
     lib = load_library()
     rows, H = _rows_alike("swiglu_forward_mx8", gate, up, output)
-    _mx8_pair("swiglu_forward_mx8", codes, scales)
-    if codes.shape != (2, *gate.shape):
-        raise ValueError("swiglu_forward_mx8: codes [2, ...] of the operands' shape")
-    with _Launch(gate, up, output, codes, scales) as L:
-        c, s, blocks = _ptr(codes), _ptr(scales), mx8_blocks(H)
-        n = rows * H
+    scales, _ = _kept_parts("swiglu_forward_mx8", kept, 2 * rows, H, False)
+    if rows == 0 or H == 0:
+        return
+    with _Launch(gate, up, output, kept) as L:
+        c, blocks = _ptr(kept), mx8_blocks(H)
+        s = c + scales
         _check(
-            lib.ck_swiglu_forward_mx8(_ptr(gate), _ptr(up), H, _ptr(output), c, c + n if n else c, H, s,
-                                      s + rows * blocks if n else s, blocks, rows, H, dtype_code(gate.dtype), L.stream),
+            lib.ck_swiglu_forward_mx8(_ptr(gate), _ptr(up), H, _ptr(output), c, c + rows * H, H, s, s + rows * blocks,
+                                      blocks, rows, H, dtype_code(gate.dtype), L.stream),
             "ck_swiglu_forward_mx8",
         )
 
 
-def swiglu_backward_mx8(codes, scales, output_grad, gate_grad, up_grad) -> None:
+def swiglu_backward_mx8(kept, output_grad, gate_grad, up_grad) -> None:
     lib = load_library()
     rows, H = _rows_alike("swiglu_backward_mx8", output_grad, gate_grad, up_grad)
-    _mx8_pair("swiglu_backward_mx8", codes, scales)
-    if codes.shape != (2, *output_grad.shape):
-        raise ValueError("swiglu_backward_mx8: codes [2, ...] of the operands' shape")
-    with _Launch(codes, scales, output_grad, gate_grad, up_grad) as L:
-        c, s, blocks = _ptr(codes), _ptr(scales), mx8_blocks(H)
-        n = rows * H
+    scales, _ = _kept_parts("swiglu_backward_mx8", kept, 2 * rows, H, False)
+    if rows == 0 or H == 0:
+        return
+    with _Launch(kept, output_grad, gate_grad, up_grad) as L:
+        c, blocks = _ptr(kept), mx8_blocks(H)
+        s = c + scales
         _check(
-            lib.ck_swiglu_backward_mx8(c, c + n if n else c, H, s, s + rows * blocks if n else s, blocks,
-                                       _ptr(output_grad), _ptr(gate_grad), _ptr(up_grad), H, None, rows, H,
-                                       dtype_code(output_grad.dtype), L.stream),
+            lib.ck_swiglu_backward_mx8(c, c + rows * H, H, s, s + rows * blocks, blocks, _ptr(output_grad),
+                                       _ptr(gate_grad), _ptr(up_grad), H, None, rows, H, dtype_code(output_grad.dtype),
+                                       L.stream),
             "ck_swiglu_backward_mx8",
         )
 
 
-def _unchunked_operands(what: str, whole, half, codes, scales, activation) -> tuple[int, int]:
+def _unchunked_rows(what: str, whole, half, activation) -> tuple[int, int]:
     rows, H = _rows_alike(what, half, activation)
-    _rows_alike(what, whole)
-    _mx8_pair(what, codes, scales)
-    lead = half.shape[:-1]
-    if whole.dtype != half.dtype or whole.shape != (*lead, 2 * H) or codes.shape != (*lead, 2, H):
-        raise ValueError(f"{what}: rows of 2 H beside rows of H, codes [..., 2, H]")
+    if whole.dtype != half.dtype or whole.shape != (*half.shape[:-1], 2 * H) or not whole.is_contiguous():
+        raise ValueError(f"{what}: contiguous rows of 2 H beside rows of H, of one dtype")
     return rows, H
 
 
-def swiglu_unchunked_forward_mx8(x, output, codes, scales) -> None:
-    """x [..., 2 H] = (up | gate); codes [..., 2, H] and scales [..., 2, ceil(H / 32)]: each half has blocks of its own."""
+def swiglu_unchunked_forward_mx8(x, output, kept) -> None:
+    """x [..., 2 H] = (up | gate); kept: rows of H, up's and gate's of a row of x behind one another."""
     lib = load_library()
-    rows, H = _unchunked_operands("swiglu_unchunked_forward_mx8", x, output, codes, scales, None)
+    rows, H = _unchunked_rows("swiglu_unchunked_forward_mx8", x, output, None)
+    scales, _ = _kept_parts("swiglu_unchunked_forward_mx8", kept, 2 * rows, H, False)
     if rows == 0 or H == 0:
         return
-    with _Launch(x, output, codes, scales) as L:
-        up, c, s, blocks = _ptr(x), _ptr(codes), _ptr(scales), mx8_blocks(H)
+    with _Launch(x, output, kept) as L:
+        up, c, blocks = _ptr(x), _ptr(kept), mx8_blocks(H)
+        s = c + scales
         _check(
             lib.ck_swiglu_forward_mx8(up + H * x.element_size(), up, 2 * H, _ptr(output), c + H, c, 2 * H, s + blocks, s,
                                       2 * blocks, rows, H, dtype_code(x.dtype), L.stream),
@@ -1050,13 +1068,15 @@ def swiglu_unchunked_forward_mx8(x, output, codes, scales) -> None:
         )
 
 
-def swiglu_unchunked_backward_mx8(codes, scales, output_grad, x_grad, activation=None) -> None:
+def swiglu_unchunked_backward_mx8(kept, output_grad, x_grad, activation=None) -> None:
     lib = load_library()
-    rows, H = _unchunked_operands("swiglu_unchunked_backward_mx8", x_grad, output_grad, codes, scales, activation)
+    rows, H = _unchunked_rows("swiglu_unchunked_backward_mx8", x_grad, output_grad, activation)
+    scales, _ = _kept_parts("swiglu_unchunked_backward_mx8", kept, 2 * rows, H, False)
     if rows == 0 or H == 0:
         return
-    with _Launch(codes, scales, output_grad, x_grad, activation) as L:
-        d_up, c, s, blocks = _ptr(x_grad), _ptr(codes), _ptr(scales), mx8_blocks(H)
+    with _Launch(kept, output_grad, x_grad, activation) as L:
+        d_up, c, blocks = _ptr(x_grad), _ptr(kept), mx8_blocks(H)
+        s = c + scales
         _check(
             lib.ck_swiglu_backward_mx8(c + H, c, 2 * H, s + blocks, s, 2 * blocks, _ptr(output_grad),
                                        d_up + H * x_grad.element_size(), d_up, 2 * H, _ptr(activation), rows, H,
@@ -1065,27 +1085,28 @@ def swiglu_unchunked_backward_mx8(codes, scales, output_grad, x_grad, activation
         )
 
 
-def _norm_vectors(what: str, dtype, B: int, H: int, rstd, *weights) -> None:
+def _norm_vectors(what: str, dtype, H: int, *weights) -> None:
     for t in weights:
         if t is not None and (t.dtype != dtype or t.numel() != H or not t.is_contiguous()):
             raise ValueError(f"{what}: weight and its gradient are dense [H] of the rows' dtype")
-    if rstd.dtype != torch.float32 or rstd.numel() != B or not rstd.is_contiguous():
-        raise ValueError(f"{what}: rstd is dense fp32 [rows]")
 
 
-def rmsnorm_forward_mx8(x, residual, weight, output, residual_out, codes, scales, rstd, eps: float) -> None:
+def rmsnorm_forward_mx8(x, residual, weight, output, residual_out, kept, eps: float) -> None:
     """Rows of x (+ residual, whose sum goes to residual_out) normalised, and kept in 8 bits with their 1 / rms."""
     lib = load_library()
     what = "rmsnorm_forward_mx8"
     B, H = _rows_alike(what, x, residual, output, residual_out)
-    _norm_vectors(what, x.dtype, B, H, rstd, weight)
-    _mx8_pair(what, codes, scales)
-    if codes.shape != x.shape or (residual is None) != (residual_out is None):
-        raise ValueError(f"{what}: codes of the shape of x, residual_out with a residual")
-    with _Launch(x, residual, weight, output, residual_out, codes, scales, rstd) as L:
+    _norm_vectors(what, x.dtype, H, weight)
+    scales, rstd = _kept_parts(what, kept, B, H, True)
+    if (residual is None) != (residual_out is None):
+        raise ValueError(f"{what}: residual_out goes with a residual")
+    if B == 0 or H == 0:
+        return
+    with _Launch(x, residual, weight, output, residual_out, kept) as L:
+        c = _ptr(kept)
         _check(
-            lib.ck_rmsnorm_forward_mx8(_ptr(x), _ptr(residual), _ptr(weight), _ptr(output), _ptr(residual_out),
-                                       _ptr(codes), _ptr(scales), _ptr(rstd), B, H, eps, dtype_code(x.dtype), L.stream),
+            lib.ck_rmsnorm_forward_mx8(_ptr(x), _ptr(residual), _ptr(weight), _ptr(output), _ptr(residual_out), c,
+                                       c + scales, c + rstd, B, H, eps, dtype_code(x.dtype), L.stream),
             "ck_rmsnorm_forward_mx8",
         )
 
@@ -1099,20 +1120,21 @@ def rmsnorm_backward_mx8_workspace_size(B: int, H: int, dtype: torch.dtype, devi
         return lib.ck_rmsnorm_backward_mx8_workspace_size(B, H, dtype_code(dtype))
 
 
-def rmsnorm_backward_mx8(codes, scales, weight, output_grad, rstd, sum_grad, x_grad, weight_grad, workspace) -> None:
+def rmsnorm_backward_mx8(kept, weight, output_grad, sum_grad, x_grad, weight_grad, workspace) -> None:
     lib = load_library()
     what = "rmsnorm_backward_mx8"
     B, H = _rows_alike(what, output_grad, sum_grad, x_grad)
-    _norm_vectors(what, output_grad.dtype, B, H, rstd, weight, weight_grad)
-    _mx8_pair(what, codes, scales)
-    if codes.shape != output_grad.shape or (weight is None) != (weight_grad is None):
-        raise ValueError(f"{what}: codes of the shape of output_grad, weight_grad with a weight")
-    with _Launch(codes, scales, weight, output_grad, rstd, sum_grad, x_grad, weight_grad, workspace) as L:
+    _norm_vectors(what, output_grad.dtype, H, weight, weight_grad)
+    scales, rstd = _kept_parts(what, kept, B, H, True)
+    if (weight is None) != (weight_grad is None):
+        raise ValueError(f"{what}: weight_grad goes with a weight")
+    with _Launch(kept, weight, output_grad, sum_grad, x_grad, weight_grad, workspace) as L:
+        c = _ptr(kept) or 0
         _check(
             lib.ck_rmsnorm_backward_mx8(
-                _ptr(codes), _ptr(scales), _ptr(weight), _ptr(output_grad), _ptr(rstd), _ptr(sum_grad), _ptr(x_grad),
-                _ptr(weight_grad), _ptr(workspace), 0 if workspace is None else workspace.numel(), B, H,
-                dtype_code(output_grad.dtype), L.stream),
+                c, c + scales, _ptr(weight), _ptr(output_grad), c + rstd, _ptr(sum_grad), _ptr(x_grad), _ptr(weight_grad),
+                _ptr(workspace), 0 if workspace is None else workspace.numel(), B, H, dtype_code(output_grad.dtype),
+                L.stream),
             "ck_rmsnorm_backward_mx8",
         )
 

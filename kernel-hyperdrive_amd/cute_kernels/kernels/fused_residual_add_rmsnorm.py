@@ -134,10 +134,10 @@ class _FusedResidualAddRMSNormMX8_Cute(torch.autograd.Function):
     def forward(
         ctx, x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None, eps: float | None
     ) -> tuple[torch.Tensor, torch.Tensor]:
-        output, residual_output, kept = rmsnorm_forward_mx8(
+        output, residual_output, saved = rmsnorm_forward_mx8(
             x.contiguous(), residual.contiguous(), None if weight is None else weight.contiguous(), eps
         )
-        ctx.save_for_backward(*kept)
+        ctx.save_for_backward(*saved)
         ctx.set_materialize_grads(False)
         return output, residual_output
 
@@ -145,7 +145,7 @@ class _FusedResidualAddRMSNormMX8_Cute(torch.autograd.Function):
     def backward(ctx, output_grad: torch.Tensor | None, residual_output_grad: torch.Tensor | None):
         if output_grad is None:
             # only the sum was used: the normalisation has no gradient
-            weight = ctx.saved_tensors[2]
+            weight = ctx.saved_tensors[1]
             return residual_output_grad, residual_output_grad, None if weight is None else torch.zeros_like(weight), None
         x_grad, weight_grad = rmsnorm_backward_mx8(ctx.saved_tensors, output_grad, residual_output_grad)
         # the sum hands the same gradient to both of its terms

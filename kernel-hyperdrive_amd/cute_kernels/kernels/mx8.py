@@ -53,6 +53,22 @@ def new_mx8(shape, device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
     )
 
 
+def new_kept(rows: int, H: int, device: torch.device, with_rstd: bool = False) -> torch.Tensor:
+    """Memory for what an operator keeps of ``rows`` rows of H elements: one buffer, laid out by ``_C.mx8_kept_offsets``."""
+    return torch.empty(_C.mx8_kept_offsets(rows, H, with_rstd)[2], dtype=torch.int8, device=device)
+
+
+def kept_pair(kept: torch.Tensor, shape) -> tuple[torch.Tensor, torch.Tensor]:
+    """The codes and scale bytes inside a buffer of ``new_kept`` for rows that lie in this shape."""
+    H = shape[-1]
+    rows = 1
+    for n in shape[:-1]:
+        rows *= n
+    start, end, _ = _C.mx8_kept_offsets(rows, H, False)
+    codes = kept[: rows * H].view(shape)
+    return codes, kept[start:end].view(torch.uint8).view(*shape[:-1], _C.mx8_blocks(H))
+
+
 @cute_op(f"{LIBRARY_NAME}::mx8_quantize_hip", mutates_args={"codes", "scales"})
 def mx8_quantize_hip(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> None:
     _C.mx8_quantize(x, codes, scales)

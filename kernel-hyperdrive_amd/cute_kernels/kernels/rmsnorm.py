@@ -19,7 +19,7 @@ from ..cutotune import CutoTuneConfig, CutoTuneParameter, cutotune, get_cartesia
 from ..enums import KernelBackend
 from ..utils import cute_op, ensure_contiguous
 from ._common import check_backend
-from .mx8 import new_mx8
+from .mx8 import new_kept
 
 
 def rmsnorm_torch(x: torch.Tensor, weight: torch.Tensor | None, eps: float | None) -> torch.Tensor:
@@ -234,31 +234,24 @@ class _RMSNorm_Cute(torch.autograd.Function):
         return x_grad, weight_grad, None, None, None, None, None, None, None, None
 
 
-@cute_op(
-    f"{LIBRARY_NAME}::rmsnorm_forward_mx8_hip",
-    mutates_args={"output", "residual_output", "codes", "scales", "rmsnorm_denominator"},
-)
+@cute_op(f"{LIBRARY_NAME}::rmsnorm_forward_mx8_hip", mutates_args={"output", "residual_output", "kept"})
 def rmsnorm_forward_mx8_hip(
     x: torch.Tensor,
     residual: torch.Tensor | None,
     weight: torch.Tensor | None,
     output: torch.Tensor,
     residual_output: torch.Tensor | None,
-    codes: torch.Tensor,
-    scales: torch.Tensor,
-    rmsnorm_denominator: torch.Tensor,
+    kept: torch.Tensor,
     eps: float,
 ) -> None:
-    _C.rmsnorm_forward_mx8(x, residual, weight, output, residual_output, codes, scales, rmsnorm_denominator, eps)
+    _C.rmsnorm_forward_mx8(x, residual, weight, output, residual_output, kept, eps)
 
 
 @cute_op(f"{LIBRARY_NAME}::rmsnorm_backward_mx8_hip", mutates_args={"x_grad", "weight_grad"})
 def rmsnorm_backward_mx8_hip(
-    codes: torch.Tensor,
-    scales: torch.Tensor,
+    kept: torch.Tensor,
     weight: torch.Tensor | None,
     output_grad: torch.Tensor,
-    rmsnorm_denominator: torch.Tensor,
     sum_grad: torch.Tensor | None,
     x_grad: torch.Tensor,
     weight_grad: torch.Tensor | None,
@@ -266,13 +259,12 @@ def rmsnorm_backward_mx8_hip(
     workspace = None
     if weight is not None:
         # fp32 partial rows of the dweight sum; taken from torch's caching allocator
+        H = weight.size(0)
         nbytes = _C.rmsnorm_backward_mx8_workspace_size(
-            rmsnorm_denominator.numel(), weight.numel(), weight.dtype, weight.device
+            output_grad.numel() // H if H > 0 else 0, H, weight.dtype, weight.device
         )
         workspace = torch.empty(max(nbytes, 16), device=weight.device, dtype=torch.uint8)
-    _C.rmsnorm_backward_mx8(
-        codes, scales, weight, output_grad, rmsnorm_denominator, sum_grad, x_grad, weight_grad, workspace
-    )
+    _C.rmsnorm_backward_mx8(kept, weight, output_grad, sum_grad, x_grad, weight_grad, workspace)
 
 
 def _keeps_8bit(x: torch.Tensor, weight: torch.Tensor | None, memory_efficient: bool, *others: torch.Tensor) -> bool:
@@ -296,46 +288,21 @@ def rmsnorm_forward_mx8(x, residual, weight, eps):
         eps = torch.finfo(x.dtype).eps
     output = torch.empty_like(x)
     residual_output = None if residual is None else torch.empty_like(x)
-    rows = x
-    if x.dim() == 1:
-        rows, residual = x.unsqueeze(0), None if residual is None else residual.unsqueeze(0)
-    codes, scales = new_mx8(rows.shape, x.device)
-    hidden_size = x.size(-1)
-    num_rows = x.numel() // hidden_size if hidden_size > 0 else 0
-    rmsnorm_denominator = torch.empty(num_rows, device=x.device, dtype=torch.float32)
-    rmsnorm_forward_mx8_hip(
-        rows,
-        residual,
-        weight,
-        output.view(rows.shape) if rows is not x else output,
-        residual_output.view(rows.shape) if rows is not x and residual is not None else residual_output,
-        codes,
-        scales,
-        rmsnorm_denominator,
-        eps,
-    )
-    return output, residual_output, (codes, scales, weight, rmsnorm_denominator)
+    H = x.size(-1)
+    kept = new_kept(x.numel() // H if H > 0 else 0, H, x.device, True)
+    rmsnorm_forward_mx8_hip(x, residual, weight, output, residual_output, kept, eps)
+    return output, residual_output, (kept, weight)
 
 
-def rmsnorm_backward_mx8(kept, output_grad, sum_grad):
+def rmsnorm_backward_mx8(saved, output_grad, sum_grad):
     """(gradient of the normalised rows, plus ``sum_grad`` where there is one, rounded once; the weight's)."""
-    codes, scales, weight, rmsnorm_denominator = kept
+    kept, weight = saved
     output_grad = output_grad.contiguous()
     if sum_grad is not None:
         sum_grad = sum_grad.contiguous()
     x_grad = torch.empty_like(output_grad)
     weight_grad = None if weight is None else torch.empty_like(weight)
-    is_1d = output_grad.dim() == 1
-    rmsnorm_backward_mx8_hip(
-        codes,
-        scales,
-        weight,
-        output_grad.unsqueeze(0) if is_1d else output_grad,
-        rmsnorm_denominator,
-        sum_grad.unsqueeze(0) if is_1d and sum_grad is not None else sum_grad,
-        x_grad.unsqueeze(0) if is_1d else x_grad,
-        weight_grad,
-    )
+    rmsnorm_backward_mx8_hip(kept, weight, output_grad, sum_grad, x_grad, weight_grad)
     return x_grad, weight_grad
 
 
@@ -344,8 +311,8 @@ class _RMSNormMX8_Cute(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x: torch.Tensor, weight: torch.Tensor | None, eps: float | None) -> torch.Tensor:
-        output, _, kept = rmsnorm_forward_mx8(x.contiguous(), None, None if weight is None else weight.contiguous(), eps)
-        ctx.save_for_backward(*kept)
+        output, _, saved = rmsnorm_forward_mx8(x.contiguous(), None, None if weight is None else weight.contiguous(), eps)
+        ctx.save_for_backward(*saved)
         return output
 
     @staticmethod

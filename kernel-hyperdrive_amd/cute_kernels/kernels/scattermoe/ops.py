@@ -31,7 +31,7 @@ from ... import _C
 from ...constants import LIBRARY_NAME
 from ...cutotune import CutoTuneConfig, CutoTuneParameter, cutotune, get_cartesian_product_cutotune_configs
 from ...utils import cute_op
-from ..mx8 import mx8_dequantize_hip, mx8_quantize_hip, new_mx8
+from ..mx8 import kept_pair, mx8_dequantize_hip, mx8_quantize_hip, new_kept, new_mx8
 from ..swiglu_unchunked import swiglu_unchunked_backward_mx8_hip
 
 
@@ -537,8 +537,8 @@ class _ScatteredGLUExpertsMX8(torch.autograd.Function):
             FAN_OUT=k,
             x_grouped=False,
         )
-        h_codes, h_scales = new_mx8((num_slots, 2, half), x.device)
-        mx8_quantize_hip(h.view(num_slots, 2, half), h_codes, h_scales)
+        h_kept = new_kept(2 * num_slots, half, x.device)
+        mx8_quantize_hip(h.view(num_slots, 2, half), *kept_pair(h_kept, (num_slots, 2, half)))
         del h
         expanded = torch.empty(num_slots, w_proj.size(-1), device=x.device, dtype=x.dtype)
         scatter2scatter(
@@ -561,16 +561,16 @@ class _ScatteredGLUExpertsMX8(torch.autograd.Function):
         x_codes, x_scales = new_mx8(x.shape, x.device)
         mx8_quantize_hip(x, x_codes, x_scales)
         ctx.save_for_backward(
-            w_fc, w_proj, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates, x_codes, x_scales, h_codes,
-            h_scales, y_codes, y_scales
+            w_fc, w_proj, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates, x_codes, x_scales, h_kept,
+            y_codes, y_scales
         )
         ctx.k = k
         return output
 
     @staticmethod
     def backward(ctx, grad_out):
-        (w_fc, w_proj, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates, x_codes, x_scales, h_codes,
-         h_scales, y_codes, y_scales) = ctx.saved_tensors
+        (w_fc, w_proj, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates, x_codes, x_scales, h_kept,
+         y_codes, y_scales) = ctx.saved_tensors
         k = ctx.k
         E = w_fc.size(0)
         num_slots, half = sorted_expert_idxs.size(0), w_proj.size(1)
@@ -604,9 +604,7 @@ class _ScatteredGLUExpertsMX8(torch.autograd.Function):
         # one pass over the kept h gives its gradient and, again, the activation
         d_h = torch.empty(num_slots, 2 * half, device=device, dtype=dtype)
         act = torch.empty(num_slots, half, device=device, dtype=dtype)
-        swiglu_unchunked_backward_mx8_hip(
-            codes=h_codes, scales=h_scales, output_grad=d_act, x_grad=d_h, activation=act
-        )
+        swiglu_unchunked_backward_mx8_hip(h_kept, d_act, d_h, act)
         del d_act
         d_w_proj = torch.empty_like(w_proj)
         group_bwd_W(DY=grouped_grad_out, X=act, expert_offsets=expert_offsets, DW=d_w_proj, E=E)

@@ -14,7 +14,7 @@ from ..cutotune import CutoTuneConfig, CutoTuneParameter, cutotune, get_cartesia
 from ..enums import KernelBackend
 from ..utils import cute_op, ensure_contiguous
 from ._common import check_backend, workgroup_size
-from .mx8 import new_mx8
+from .mx8 import new_kept
 
 
 def swiglu_torch(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
@@ -97,40 +97,37 @@ class _Swiglu_Cute(torch.autograd.Function):
         return gate_grad, up_grad, None, None, None, None
 
 
-@cute_op(f"{LIBRARY_NAME}::swiglu_forward_mx8_hip", mutates_args={"output", "codes", "scales"})
-def swiglu_forward_mx8_hip(
-    gate: torch.Tensor, up: torch.Tensor, output: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor
-) -> None:
-    _C.swiglu_forward_mx8(gate, up, output, codes, scales)
+@cute_op(f"{LIBRARY_NAME}::swiglu_forward_mx8_hip", mutates_args={"output", "kept"})
+def swiglu_forward_mx8_hip(gate: torch.Tensor, up: torch.Tensor, output: torch.Tensor, kept: torch.Tensor) -> None:
+    _C.swiglu_forward_mx8(gate, up, output, kept)
 
 
 @cute_op(f"{LIBRARY_NAME}::swiglu_backward_mx8_hip", mutates_args={"gate_grad", "up_grad"})
 def swiglu_backward_mx8_hip(
-    codes: torch.Tensor, scales: torch.Tensor, output_grad: torch.Tensor, gate_grad: torch.Tensor, up_grad: torch.Tensor
+    kept: torch.Tensor, output_grad: torch.Tensor, gate_grad: torch.Tensor, up_grad: torch.Tensor
 ) -> None:
-    _C.swiglu_backward_mx8(codes, scales, output_grad, gate_grad, up_grad)
+    _C.swiglu_backward_mx8(kept, output_grad, gate_grad, up_grad)
 
 
 class _SwigluMX8_Cute(torch.autograd.Function):
-    """As ``_Swiglu_Cute``, with gate and up saved in 8 bits (see mx8.py) by the forward's own pass: codes and scale bytes of
-    the two behind one another."""
+    """As ``_Swiglu_Cute``, with gate and up saved in 8 bits (see mx8.py) by the forward's own pass."""
 
     @staticmethod
     def forward(ctx, gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
         gate, up = gate.contiguous(), up.contiguous()
         output = torch.empty_like(gate)
-        codes, scales = new_mx8((2, *gate.shape), gate.device)
-        swiglu_forward_mx8_hip(gate, up, output, codes, scales)
-        ctx.save_for_backward(codes, scales)
+        H = gate.size(-1)
+        kept = new_kept(2 * gate.numel() // H if H > 0 else 0, H, gate.device)
+        swiglu_forward_mx8_hip(gate, up, output, kept)
+        ctx.save_for_backward(kept)
         return output
 
     @staticmethod
     def backward(ctx, output_grad: torch.Tensor):
-        codes, scales = ctx.saved_tensors
         output_grad = output_grad.contiguous()
         gate_grad = torch.empty_like(output_grad)
         up_grad = torch.empty_like(output_grad)
-        swiglu_backward_mx8_hip(codes, scales, output_grad, gate_grad, up_grad)
+        swiglu_backward_mx8_hip(ctx.saved_tensors[0], output_grad, gate_grad, up_grad)
         return gate_grad, up_grad
 
 

@@ -15,7 +15,7 @@ from ..enums import KernelBackend
 from ..math import divide_if_divisible
 from ..utils import cute_op, ensure_contiguous
 from ._common import check_backend, workgroup_size
-from .mx8 import new_mx8
+from .mx8 import new_kept
 
 
 def swiglu_unchunked_torch(x: torch.Tensor) -> torch.Tensor:
@@ -97,23 +97,17 @@ class _SwigluUnchunked_Cute(torch.autograd.Function):
         return x_grad, None, None, None, None, None, None
 
 
-@cute_op(f"{LIBRARY_NAME}::swiglu_unchunked_forward_mx8_hip", mutates_args={"output", "codes", "scales"})
-def swiglu_unchunked_forward_mx8_hip(
-    x: torch.Tensor, output: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor
-) -> None:
-    _C.swiglu_unchunked_forward_mx8(x, output, codes, scales)
+@cute_op(f"{LIBRARY_NAME}::swiglu_unchunked_forward_mx8_hip", mutates_args={"output", "kept"})
+def swiglu_unchunked_forward_mx8_hip(x: torch.Tensor, output: torch.Tensor, kept: torch.Tensor) -> None:
+    _C.swiglu_unchunked_forward_mx8(x, output, kept)
 
 
 @cute_op(f"{LIBRARY_NAME}::swiglu_unchunked_backward_mx8_hip", mutates_args={"x_grad", "activation"})
 def swiglu_unchunked_backward_mx8_hip(
-    codes: torch.Tensor,
-    scales: torch.Tensor,
-    output_grad: torch.Tensor,
-    x_grad: torch.Tensor,
-    activation: torch.Tensor | None = None,
+    kept: torch.Tensor, output_grad: torch.Tensor, x_grad: torch.Tensor, activation: torch.Tensor | None = None
 ) -> None:
     """``activation``: also written, with the forward's output at the kept inputs."""
-    _C.swiglu_unchunked_backward_mx8(codes, scales, output_grad, x_grad, activation)
+    _C.swiglu_unchunked_backward_mx8(kept, output_grad, x_grad, activation)
 
 
 class _SwigluUnchunkedMX8_Cute(torch.autograd.Function):
@@ -125,18 +119,17 @@ class _SwigluUnchunkedMX8_Cute(torch.autograd.Function):
         *lead, H = x.shape
         h = divide_if_divisible(H, 2, "last dimension of x must be even")
         output = torch.empty((*lead, h), device=x.device, dtype=x.dtype)
-        codes, scales = new_mx8((*lead, 2, h), x.device)
-        swiglu_unchunked_forward_mx8_hip(x, output, codes, scales)
-        ctx.save_for_backward(codes, scales)
+        kept = new_kept(x.numel() // h if h > 0 else 0, h, x.device)
+        swiglu_unchunked_forward_mx8_hip(x, output, kept)
+        ctx.save_for_backward(kept)
         return output
 
     @staticmethod
     def backward(ctx, output_grad: torch.Tensor):
-        codes, scales = ctx.saved_tensors
         output_grad = output_grad.contiguous()
         *lead, h = output_grad.shape
         x_grad = torch.empty((*lead, 2 * h), device=output_grad.device, dtype=output_grad.dtype)
-        swiglu_unchunked_backward_mx8_hip(codes, scales, output_grad, x_grad)
+        swiglu_unchunked_backward_mx8_hip(ctx.saved_tensors[0], output_grad, x_grad)
         return x_grad
 
 

@@ -256,16 +256,16 @@ def test_swiglu_unchunked(gpu, dtype, shape):
 def test_swiglu_activation_is_recomputed_at_the_kept_values(gpu, dtype):
     """What the experts' backward takes from the same pass.  fp32 evaluation: as for the forward, 2^-19."""
     from cute_kernels import _C
-    from cute_kernels.kernels.mx8 import new_mx8
+    from cute_kernels.kernels.mx8 import kept_pair, new_kept
 
     announce("swiglu activation", dtype)
     for rows, h in [(5, 32), (5, 37), (65, 136)]:
         x, dy = rows_like_activations((rows, 2 * h), dtype, 10), randn((rows, h), dtype, 11)
-        codes, scales = new_mx8((rows, 2, h), gpu)
-        _C.mx8_quantize(x.to(gpu).view(rows, 2, h), codes, scales)
+        kept = new_kept(2 * rows, h, gpu)
+        _C.mx8_quantize(x.to(gpu).view(rows, 2, h), *kept_pair(kept, (rows, 2, h)))
         dx = torch.empty(rows, 2 * h, dtype=dtype, device=gpu)
         act = torch.empty(rows, h, dtype=dtype, device=gpu)
-        _C.swiglu_unchunked_backward_mx8(codes, scales, dy.to(gpu), dx, act)
+        _C.swiglu_unchunked_backward_mx8(kept, dy.to(gpu), dx, act)
         up, gate = x.chunk(2, dim=-1)
         assert_rounded(act, swiglu64(kept64(gate.contiguous()), kept64(up.contiguous())), dtype, 2.0 ** -19, what="act",
                        lost=2.0 ** -126 * (kept64(gate.contiguous()) * kept64(up.contiguous())).abs())
