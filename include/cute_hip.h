@@ -346,17 +346,17 @@ int ck_expert_bias_backward(const void* dy, int64_t dy_stride, const int64_t* ex
  *   d logits = m p [ g_b E / N (f_e - sum_j f_j p_tj) + g_z 2 / N lse_t ],  f_e = c_e / (N k)
  *   logits [tokens, E], rows `ld` elements apart; selected int64 [tokens, k] (ids outside [0, E) count nowhere); mask one
  *   byte per token (non-zero counts).  Masked rows may hold anything; N = 0 gives zeros; a row of
- *   nothing but -inf or the type's lowest value has no probabilities and no lse.  balance, z: one fp32 each; counts int32 [E]; stats int32 [2] (N, counted selections), read by the
- *   backward.  balance_grad / z_grad: one fp32 each on the device, or NULL for zero.  d_logits dense [tokens, E].
+ *   nothing but -inf or the type's lowest value has no probabilities and no lse.  balance, z: one fp32 each; counts int32 [E]; shares fp32 [E + 1], for the backward:
+ *   E / N (f_e - mean f) and 1 / N.  balance_grad / z_grad: one fp32 each on the device, or NULL for zero.  d_logits dense [tokens, E].
  * E <= 1024, 1 <= k <= E, tokens * k < 2^31.  Sums in fp32 per workgroup, in fp64 over them, in a fixed order.
  * ------------------------------------------------------------------------------------------- */
 int64_t ck_moe_balance_loss_workspace_size(int64_t tokens, int64_t E);
 int ck_moe_balance_loss_forward(const void* logits, int64_t ld, const int64_t* selected, const void* mask, float* balance,
-                                float* z, int* counts, int* stats, void* workspace, int64_t workspace_bytes,
+                                float* z, int* counts, float* shares, void* workspace, int64_t workspace_bytes,
                                 int64_t tokens, int64_t E, int64_t k, int dtype, void* stream);
-int ck_moe_balance_loss_backward(const void* logits, int64_t ld, const void* mask, const int* counts, const int* stats,
+int ck_moe_balance_loss_backward(const void* logits, int64_t ld, const void* mask, const float* shares,
                                  const float* balance_grad, const float* z_grad, void* d_logits, int64_t tokens, int64_t E,
-                                 int64_t k, int dtype, void* stream);
+                                 int dtype, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Activations kept in 8 bits between forward and backward (no counterpart in the reference): MXINT8 of the OCP

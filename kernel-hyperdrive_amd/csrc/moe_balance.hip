@@ -9,7 +9,8 @@
 // write partial sums; a second launch of one workgroup adds them up in a fixed order (no floating-point atomics; the
 // counts are whole numbers).  Few tokens take one workgroup that finishes by itself.
 // f_e - sum f p cancels when the load is balanced.  The probabilities sum to one, so any constant may be taken off f
-// first: f_e - mean f = (E c_e - sum c) / (N k E) comes from whole numbers and loses nothing.
+// first: f_e - mean f = (E c_e - sum c) / (N k E) comes from whole numbers and loses nothing.  The forward leaves E / N times
+// that for every expert, and 1 / N behind them, for the backward (`shares`).
 #include "ck_piece.h"
 
 namespace ck {
@@ -17,22 +18,52 @@ namespace ck {
 constexpr int kBalanceMaxExperts = 1024;
 constexpr int kPiece = 8;  // experts a lane holds side by side
 
-template <int LPT>
-__device__ __forceinline__ float group_max(float v) {
-#pragma unroll
-    for (int off = 1; off < LPT; off <<= 1) v = fmaxf(v, __shfl_xor(v, off, CK_WAVE));
+// Combines a value over the LPT neighbouring lanes that hold a token's row, in all of them.  Up to sixteen lanes by register
+// exchanges (quad_perm 1 0 3 2, quad_perm 2 3 0 1; behind those the quads are uniform, so the mirror images of eight and of
+// sixteen lanes bring the other half's value), beyond by shuffles.
+template <int CTRL>
+__device__ __forceinline__ float lanes_moved(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+}
+template <int LPT, typename F>
+__device__ __forceinline__ float group_reduce(float v, F&& op) {
+    if (LPT >= 2) v = op(v, lanes_moved<0xB1>(v));
+    if (LPT >= 4) v = op(v, lanes_moved<0x4E>(v));
+    if (LPT >= 8) v = op(v, lanes_moved<0x141>(v));
+    if (LPT >= 16) v = op(v, lanes_moved<0x140>(v));
+    if (LPT >= 32) v = op(v, __shfl_xor(v, 16, CK_WAVE));
+    if (LPT >= 64) v = op(v, __shfl_xor(v, 32, CK_WAVE));
     return v;
 }
 template <int LPT>
+__device__ __forceinline__ float group_max(float v) {
+    return group_reduce<LPT>(v, [](float a, float b) { return fmaxf(a, b); });
+}
+template <int LPT>
 __device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-    for (int off = 1; off < LPT; off <<= 1) v += __shfl_xor(v, off, CK_WAVE);
-    return v;
+    return group_reduce<LPT>(v, [](float a, float b) { return a + b; });
+}
+
+// exp(x) for x <= 0, -inf or NaN: 2^(x log2 e), the product's rounding error kept and applied to first order, so that the
+// result is as good at -80 as at -1.  (Below -200, where 2^.. is 0, x counts as -200: -inf has no rounding error.)
+__device__ __forceinline__ float exp_nonpositive(float x) {
+    x = x < -200.f ? -200.f : x;
+    const float log2e = 1.44269504f, log2e_rest = 1.92596299e-8f;  // log2 e = their sum to 48 bits
+    const float hi = x * log2e;
+    const float lo = fmaf(x, log2e, -hi) + x * log2e_rest;
+    const float e = __builtin_amdgcn_exp2f(hi);
+    return fmaf(e, lo * 0.693147181f, e);
 }
 __device__ __forceinline__ double wave_sum_d(double v) {
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, CK_WAVE);
     return v;
+}
+
+// experts a piece that starts at column `col` holds
+__device__ __forceinline__ int piece_size(int E, int col) {
+    const int left = E - col;
+    return left >= kPiece ? kPiece : (left > 0 ? left : 0);
 }
 
 // lowest finite value of a storage type: what a mask writes where -inf is not wanted
@@ -45,18 +76,19 @@ __device__ __forceinline__ float lowest_of<F16>() { return -65504.f; }
 template <>
 __device__ __forceinline__ float lowest_of<BF16>() { return -3.3895313892515355e38f; }
 
-// Probabilities of one token from its logits, in place (columns >= E become 0), and its log-sum-exp.  A row whose mask
+// Probabilities of one token from its logits, in place (columns beyond a piece's size become 0), and its log-sum-exp.  A row whose mask
 // left nothing - -inf or the type's lowest value throughout - has no probabilities and counts as lse 0 (every exponential
 // below is then 0); a NaN, or +inf, makes the row NaN.
-template <typename T, int LPT, int CHUNKS>
-__device__ __forceinline__ float token_softmax(float (&v)[CHUNKS][kPiece], int first, int E) {
+template <typename T, int LPT, int CHUNKS, bool VEC>
+__device__ __forceinline__ float token_softmax(float (&v)[CHUNKS][kPiece], const int (&size)[CHUNKS]) {
     const float none = -__builtin_inff();
     float top = none;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
         for (int j = 0; j < kPiece; ++j) {
-            if (first + c * LPT * kPiece + j >= E) v[c][j] = none;
+            // (aligned rows have whole pieces or none)
+            if (VEC ? size[c] == 0 : j >= size[c]) v[c][j] = none;
             top = fmaxf(top, v[c][j]);
         }
     top = group_max<LPT>(top);
@@ -66,7 +98,7 @@ __device__ __forceinline__ float token_softmax(float (&v)[CHUNKS][kPiece], int f
     for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
         for (int j = 0; j < kPiece; ++j) {
-            v[c][j] = expf(v[c][j] - top);
+            v[c][j] = exp_nonpositive(v[c][j] - top);
             sum += v[c][j];
         }
     sum = group_sum<LPT>(sum);
@@ -81,8 +113,8 @@ __device__ __forceinline__ float token_softmax(float (&v)[CHUNKS][kPiece], int f
 
 // losses from the summed columns; all threads of the workgroup call it.  Thread e (< E) brings expert e's sums.
 struct BalanceOut {
-    float *balance, *z;
-    int *counts, *stats;  // stats: counting tokens, counted selections
+    float *balance, *z, *shares;
+    int* counts;
 };
 template <int WAVES>
 __device__ __forceinline__ void balance_finish(double prob, int count, double z, int tokens, int E, int k, BalanceOut out) {
@@ -100,27 +132,29 @@ __device__ __forceinline__ void balance_finish(double prob, int count, double z,
         totals[wave][0] = tokens;
         totals[wave][1] = selections;
     }
-    if (mine) out.counts[e] = count;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        double c = 0.0, zz = 0.0;
-        int n = 0, total = 0;
+    double c = 0.0, zz = 0.0;
+    int n = 0, total = 0;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-            c += sums[w][0];
-            zz += sums[w][1];
-            n += totals[w][0];
-            total += totals[w][1];
-        }
-        const double tokens_d = n > 0 ? (double)n : 1.0;
-        *out.balance = (float)((double)E * c / (tokens_d * tokens_d * (double)k));
-        *out.z = (float)(zz / tokens_d);
-        out.stats[0] = n;
-        out.stats[1] = total;
+    for (int w = 0; w < WAVES; ++w) {
+        c += sums[w][0];
+        zz += sums[w][1];
+        n += totals[w][0];
+        total += totals[w][1];
+    }
+    const double per_token = n > 0 ? 1.0 / (double)n : 0.0, scale = per_token * per_token / (double)k;
+    if (mine) {
+        out.counts[e] = count;
+        out.shares[e] = (float)(scale * (double)((long long)E * count - total));
+    }
+    if (threadIdx.x == 0) {
+        *out.balance = (float)((double)E * c * scale);
+        *out.z = (float)(zz * per_token);
+        out.shares[E] = (float)per_token;
     }
 }
 
-// Partial sums of `per_block` consecutive tokens per workgroup: prob [G][E], count [G][E], z [G], tokens [G]; ALONE: the only
+// Partial sums of `per_block` consecutive tokens per workgroup: prob and count [G][E padded to 4], z [G], tokens [G]; ALONE: the only
 // workgroup, which writes the results.
 template <typename T, int LPT, int CHUNKS, int WAVES, bool VEC, bool ALONE>
 __global__ void __launch_bounds__(WAVES * CK_WAVE)
@@ -137,12 +171,34 @@ __global__ void __launch_bounds__(WAVES * CK_WAVE)
     const int wave = threadIdx.x / CK_WAVE, lane = lane_id(), first = (lane % LPT) * kPiece;
     const int64_t t0 = (int64_t)blockIdx.x * per_block;
     const int64_t t1 = t0 + per_block < tokens ? t0 + per_block : tokens;
+    int size[CHUNKS];
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) size[c] = piece_size(E, first + c * LPT * kPiece);
+    // a turn's rows: requested first, worked on after the next turn's are on their way
+    struct Rows {
+        Piece<T, kPiece> row[CHUNKS];
+        bool real;
+    };
+    auto fetch = [&](int64_t base, Rows& r) __attribute__((always_inline)) {
+        const int64_t t = base + lane / LPT;
+        r.real = t < t1 && (mask == nullptr || mask[t] != 0);
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            r.row[c].clear();
+            if (r.real && size[c] > 0)
+                r.row[c] = load_piece<T, kPiece, VEC, false>(logits + t * ld + first + c * LPT * kPiece, size[c]);
+        }
+    };
+    int64_t base = t0 + wave * TPW;
+    Rows cur, next;
+    fetch(base, cur);
     for (int e = threadIdx.x; e < COLS; e += WAVES * CK_WAVE) count[e] = 0;
     __syncthreads();
 
     for (int64_t i = t0 * k + threadIdx.x; i < t1 * k; i += WAVES * CK_WAVE) {
         const int64_t id = selected[i];
-        if (id >= 0 && id < E && (mask == nullptr || mask[i / k] != 0)) atomicAdd(&count[id], 1);
+        if (id >= 0 && id < E && (mask == nullptr || mask[t0 + (uint32_t)(i - t0 * k) / (uint32_t)k] != 0))
+            atomicAdd(&count[id], 1);
     }
 
     float acc[CHUNKS][kPiece];
@@ -152,22 +208,15 @@ __global__ void __launch_bounds__(WAVES * CK_WAVE)
         for (int j = 0; j < kPiece; ++j) acc[c][j] = 0.f;
     float z = 0.f;
     int n = 0;
-    for (int64_t base = t0 + wave * TPW; base < t1; base += WAVES * TPW) {
-        const int64_t t = base + lane / LPT;
-        const bool real = t < t1 && (mask == nullptr || mask[t] != 0);
+    for (; base < t1; base += WAVES * TPW) {
+        fetch(base + WAVES * TPW, next);
         float v[CHUNKS][kPiece];
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-            const int col = first + c * LPT * kPiece;
-            const int left = E - col, size = left >= kPiece ? kPiece : (left > 0 ? left : 0);
-            Piece<T, kPiece> row;
-            row.clear();
-            if (real && size > 0) row = load_piece<T, kPiece, VEC, false>(logits + t * ld + col, size);
+        for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
-            for (int j = 0; j < kPiece; ++j) v[c][j] = row.up(j);
-        }
-        const float lse = token_softmax<T, LPT, CHUNKS>(v, first, E);
-        if (real) {
+            for (int j = 0; j < kPiece; ++j) v[c][j] = cur.row[c].up(j);
+        const float lse = token_softmax<T, LPT, CHUNKS, VEC>(v, size);
+        if (cur.real) {
 #pragma unroll
             for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
@@ -177,6 +226,7 @@ __global__ void __launch_bounds__(WAVES * CK_WAVE)
                 n += 1;
             }
         }
+        cur = next;
     }
     // the wave's token groups, then the waves
 #pragma unroll
@@ -208,12 +258,14 @@ __global__ void __launch_bounds__(WAVES * CK_WAVE)
         }
         balance_finish<WAVES>(p, c, zz, nn, E, k, out);
     } else {
-        for (int e = threadIdx.x; e < E; e += WAVES * CK_WAVE) {
+        // (columns up to the next multiple of four: a piece's columns beyond E hold zeros)
+        const int padded = (E + 3) & ~3;
+        for (int e = threadIdx.x; e < padded; e += WAVES * CK_WAVE) {
             float p = 0.f;
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) p += prob[w][e];
-            prob_partial[(int64_t)blockIdx.x * E + e] = p;
-            count_partial[(int64_t)blockIdx.x * E + e] = count[e];
+            prob_partial[(int64_t)blockIdx.x * padded + e] = p;
+            count_partial[(int64_t)blockIdx.x * padded + e] = count[e];
         }
         if (threadIdx.x == 0) {
             float zz = 0.f;
@@ -229,80 +281,102 @@ __global__ void __launch_bounds__(WAVES * CK_WAVE)
     }
 }
 
-// One workgroup adds the partial sums of `parts` workgroups up: 1024 / columns row groups by columns (a power of two >= E).
+// One workgroup adds the partial sums of `parts` workgroups up.  A thread owns four columns (rows of partial sums are padded
+// to `padded`, a multiple of four) and every `1024 / quads`-th row, with `quads` a power of two >= padded / 4; lanes of a
+// wave that own the same columns meet by shuffles, waves in LDS.
 __global__ void __launch_bounds__(1024)
     balance_sum_kernel(const float* __restrict__ prob_partial, const int* __restrict__ count_partial,
-                       const float* __restrict__ z_partial, const int* __restrict__ token_partial, int parts, int E, int k,
-                       int columns, BalanceOut out) {
-    __shared__ double prob[1024];
-    __shared__ int count[1024];
-    const int e = threadIdx.x % columns, group = threadIdx.x / columns, groups = 1024 / columns;
-    double p = 0.0;
-    int c = 0;
-    if (e < E) {
+                       const float* __restrict__ z_partial, const int* __restrict__ token_partial, int parts, int E,
+                       int padded, int k, int quads, BalanceOut out) {
+    __shared__ float prob[4096];  // [places][4 * quads]: 16 waves, or fewer rows of more than 64 quads
+    __shared__ int count[4096];
+    const int quad = threadIdx.x & (quads - 1), group = threadIdx.x / quads, groups = 1024 / quads;
+    float p[4] = {0.f, 0.f, 0.f, 0.f};
+    int c[4] = {0, 0, 0, 0};
+    if (quad * 4 < padded) {
+#pragma unroll 4
         for (int r = group; r < parts; r += groups) {
-            p += (double)prob_partial[(int64_t)r * E + e];
-            c += count_partial[(int64_t)r * E + e];
+            const float4 pv = *reinterpret_cast<const float4*>(prob_partial + (int64_t)r * padded + quad * 4);
+            const int4 cv = *reinterpret_cast<const int4*>(count_partial + (int64_t)r * padded + quad * 4);
+            p[0] += pv.x;
+            p[1] += pv.y;
+            p[2] += pv.z;
+            p[3] += pv.w;
+            c[0] += cv.x;
+            c[1] += cv.y;
+            c[2] += cv.z;
+            c[3] += cv.w;
         }
     }
-    prob[threadIdx.x] = p;
-    count[threadIdx.x] = c;
     double z = 0.0;
     int n = 0;
     for (int r = threadIdx.x; r < parts; r += 1024) {
         z += (double)z_partial[r];
         n += token_partial[r];
     }
-    __syncthreads();
-    p = 0.0;
-    c = 0;
-    if ((int)threadIdx.x < E) {
-        for (int g = 0; g < groups; ++g) {
-            p += prob[g * columns + threadIdx.x];
-            c += count[g * columns + threadIdx.x];
+    for (int off = quads; off < CK_WAVE; off <<= 1) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            p[j] += __shfl_xor(p[j], off, CK_WAVE);
+            c[j] += __shfl_xor(c[j], off, CK_WAVE);
         }
     }
-    balance_finish<16>(p, c, z, n, E, k, out);
+    const int place = quads < CK_WAVE ? (int)threadIdx.x / CK_WAVE : group;
+    const int places = quads < CK_WAVE ? 1024 / CK_WAVE : groups;
+    if (quads >= CK_WAVE || lane_id() < quads) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            prob[place * 4 * quads + quad * 4 + j] = p[j];
+            count[place * 4 * quads + quad * 4 + j] = c[j];
+        }
+    }
+    __syncthreads();
+    double total = 0.0;
+    int hits = 0;
+    if ((int)threadIdx.x < E) {
+        for (int g = 0; g < places; ++g) {
+            total += (double)prob[g * 4 * quads + threadIdx.x];
+            hits += count[g * 4 * quads + threadIdx.x];
+        }
+    }
+    balance_finish<16>(total, hits, z, n, E, k, out);
 }
 
 template <typename T, int LPT, int CHUNKS, bool VEC>
 __global__ void __launch_bounds__(256)
     balance_bwd_kernel(const typename T::storage_t* __restrict__ logits, int64_t ld, const uint8_t* __restrict__ mask,
-                       const int* __restrict__ counts, const int* __restrict__ stats, const float* __restrict__ balance_grad,
-                       const float* __restrict__ z_grad, typename T::storage_t* __restrict__ d_logits, int64_t tokens, int E,
-                       int k) {
+                       const float* __restrict__ shares, const float* __restrict__ balance_grad,
+                       const float* __restrict__ z_grad, typename T::storage_t* __restrict__ d_logits, int64_t tokens, int E) {
     constexpr int TPW = CK_WAVE / LPT;
     const int lane = lane_id(), first = (lane % LPT) * kPiece;
     const int64_t wave = (int64_t)blockIdx.x * 4 + threadIdx.x / CK_WAVE, waves = (int64_t)gridDim.x * 4;
-    const int n = stats[0];
-    const double per_token = n > 0 ? 1.0 / (double)n : 0.0;
-    // g_b E / N (f_e - mean f), with f_e - mean f = (E c_e - sum c) / (N k E)
-    const double scale = balance_grad != nullptr ? (double)*balance_grad * per_token * per_token / (double)k : 0.0;
-    const float z_scale = z_grad != nullptr ? (float)(2.0 * (double)*z_grad * per_token) : 0.f;
-    const long long total = stats[1];
+    const float g_b = balance_grad != nullptr ? *balance_grad : 0.f;
+    const float z_scale = z_grad != nullptr ? 2.f * *z_grad * shares[E] : 0.f;
+    int size[CHUNKS];
     float a[CHUNKS][kPiece];
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c)
+    for (int c = 0; c < CHUNKS; ++c) {
+        size[c] = piece_size(E, first + c * LPT * kPiece);
 #pragma unroll
         for (int j = 0; j < kPiece; ++j) {
             const int e = first + c * LPT * kPiece + j;
-            a[c][j] = e < E ? (float)(scale * (double)((long long)E * counts[e] - total)) : 0.f;
+            a[c][j] = e < E ? g_b * shares[e] : 0.f;
         }
+    }
     for (int64_t base = wave * TPW; base < tokens; base += waves * TPW) {
         const int64_t t = base + lane / LPT;
         const bool real = t < tokens && (mask == nullptr || mask[t] != 0);
         float v[CHUNKS][kPiece];
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-            const int col = first + c * LPT * kPiece;
-            const int left = E - col, size = left >= kPiece ? kPiece : (left > 0 ? left : 0);
             Piece<T, kPiece> row;
             row.clear();
-            if (real && size > 0) row = load_piece<T, kPiece, VEC, false>(logits + t * ld + col, size);
+            if (real && size[c] > 0)
+                row = load_piece<T, kPiece, VEC, false>(logits + t * ld + first + c * LPT * kPiece, size[c]);
 #pragma unroll
             for (int j = 0; j < kPiece; ++j) v[c][j] = row.up(j);
         }
-        const float lse = token_softmax<T, LPT, CHUNKS>(v, first, E);
+        const float lse = token_softmax<T, LPT, CHUNKS, VEC>(v, size);
         float inner = 0.f;
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c)
@@ -312,12 +386,11 @@ __global__ void __launch_bounds__(256)
         const float shift = z_scale * lse - inner;
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-            const int col = first + c * LPT * kPiece;
-            const int left = E - col, size = left >= kPiece ? kPiece : (left > 0 ? left : 0);
             Piece<T, kPiece> o;
 #pragma unroll
             for (int j = 0; j < kPiece; ++j) o.put(j, real ? v[c][j] * (a[c][j] + shift) : 0.f);
-            if (t < tokens && size > 0) store_piece<T, kPiece, VEC>(o, d_logits + t * E + col, size);
+            if (t < tokens && size[c] > 0)
+                store_piece<T, kPiece, VEC>(o, d_logits + t * E + first + c * LPT * kPiece, size[c]);
         }
     }
 }
@@ -332,15 +405,20 @@ int balance_lanes(int64_t E) {
     while (lanes < 64 && lanes * ck::kPiece < E) lanes *= 2;
     return lanes;
 }
-// tokens one workgroup of 16 waves takes alone
-int64_t balance_alone(int64_t E) { return 16 * (64 / balance_lanes(E)) * 4; }
-// Workgroups of the forward: a wave gets one or two turns, and what the adding workgroup reads stays within 64 K pairs.
+// Tokens sixteen waves hold at once
+int64_t balance_turn(int64_t E) { return 16 * (64 / balance_lanes(E)); }
+// Workgroups of the forward: a turn each, up to one per compute unit, and no more than 128 K pairs for the workgroup that
+// adds them up.  Measured (both launches): 65521 x 160 fp32 24.3 us, with twice the workgroups 27.0, with half 32.3.  One
+// workgroup alone takes up to four turns: 4096 x 8 bf16 11.2 us, against 12.1 in two launches; beyond, the two launches win
+// (8192 x 8: 12.3 against 18.6).
 int64_t balance_parts(int64_t tokens, int64_t E) {
-    if (tokens <= balance_alone(E)) return 1;
-    const int64_t wanted = ck_ceil_div(tokens, 4 * (64 / balance_lanes(E)) * 2);
-    const int64_t most = 65536 / E < 1024 ? 65536 / E : 1024;
+    if (tokens <= 4 * balance_turn(E)) return 1;
+    const int64_t wanted = ck_ceil_div(tokens, balance_turn(E));
+    const int64_t most = 131072 / E < 256 ? 131072 / E : 256;
     return wanted < most ? wanted : most;
 }
+int64_t balance_padded(int64_t E) { return (E + 3) / 4 * 4; }
+int64_t balance_workspace(int64_t parts, int64_t E) { return parts == 1 ? 0 : parts * (balance_padded(E) + 1) * 8; }
 
 struct BalanceArgs {
     const void* logits;
@@ -362,7 +440,7 @@ void balance_launch_fwd(hipStream_t s, const BalanceArgs& a) {
                            (const S*)a.logits, a.ld, a.selected, a.mask, a.tokens, a.E, a.k, a.tokens, (float*)nullptr,
                            (int*)nullptr, (float*)nullptr, (int*)nullptr, a.out);
     else
-        hipLaunchKernelGGL((ck::balance_fwd_kernel<T, LPT, CHUNKS, 4, VEC, false>), dim3((unsigned)a.parts), dim3(256), 0, s,
+        hipLaunchKernelGGL((ck::balance_fwd_kernel<T, LPT, CHUNKS, 16, VEC, false>), dim3((unsigned)a.parts), dim3(1024), 0, s,
                            (const S*)a.logits, a.ld, a.selected, a.mask, a.tokens, a.E, a.k, a.per_block, a.prob, a.count,
                            a.z, a.n, a.out);
 }
@@ -370,19 +448,18 @@ struct BalanceBwd {
     const void* logits;
     int64_t ld;
     const uint8_t* mask;
-    const int *counts, *stats;
-    const float *balance_grad, *z_grad;
+    const float *shares, *balance_grad, *z_grad;
     void* d_logits;
     int64_t tokens;
-    int E, k;
+    int E;
 };
 template <typename T, int LPT, int CHUNKS, bool VEC>
 void balance_launch_bwd(hipStream_t s, const BalanceBwd& a) {
     typedef typename T::storage_t S;
+    // (a wave reads the experts' shares once for all its turns: 65521 x 160 fp32 17.8 us with 1024 workgroups, 18.9 with 2048)
     const int64_t need = ck_ceil_div(a.tokens, 4 * (64 / LPT));
-    hipLaunchKernelGGL((ck::balance_bwd_kernel<T, LPT, CHUNKS, VEC>), dim3((unsigned)(need < 2048 ? need : 2048)), dim3(256),
-                       0, s, (const S*)a.logits, a.ld, a.mask, a.counts, a.stats, a.balance_grad, a.z_grad, (S*)a.d_logits,
-                       a.tokens, a.E, a.k);
+    hipLaunchKernelGGL((ck::balance_bwd_kernel<T, LPT, CHUNKS, VEC>), dim3((unsigned)(need < 1024 ? need : 1024)), dim3(256),
+                       0, s, (const S*)a.logits, a.ld, a.mask, a.shares, a.balance_grad, a.z_grad, (S*)a.d_logits, a.tokens, a.E);
 }
 
 #define CK_BALANCE_LANES(E, ...)                                                    \
@@ -412,19 +489,19 @@ bool balance_shape(int64_t tokens, int64_t E, int64_t k) {
 extern "C" int64_t ck_moe_balance_loss_workspace_size(int64_t tokens, int64_t E) {
     if (tokens <= 0 || E < 1 || E > ck::kBalanceMaxExperts) return 0;
     const int64_t parts = balance_parts(tokens, E);
-    return parts == 1 ? 0 : parts * (E + 1) * 8;
+    return balance_workspace(parts, E);
 }
 
 extern "C" int ck_moe_balance_loss_forward(const void* logits, int64_t ld, const int64_t* selected, const void* mask,
-                                           float* balance, float* z, int* counts, int* stats, void* workspace,
+                                           float* balance, float* z, int* counts, float* shares, void* workspace,
                                            int64_t workspace_bytes, int64_t tokens, int64_t E, int64_t k, int dtype,
                                            void* stream) {
     if (!balance_shape(tokens, E, k) || ld < E) return CK_ERR_SHAPE;
     if (dtype != CK_F32 && dtype != CK_F16 && dtype != CK_BF16) return CK_ERR_DTYPE;
-    if (!balance || !z || !counts || !stats || (tokens > 0 && (!logits || !selected))) return CK_ERR_NULL;
+    if (!balance || !z || !counts || !shares || (tokens > 0 && (!logits || !selected))) return CK_ERR_NULL;
     if (!ck_aligned_elem(logits, dtype)) return CK_ERR_ALIGN;
     const int64_t parts = balance_parts(tokens, E);
-    const int64_t need = parts == 1 ? 0 : parts * (E + 1) * 8;
+    const int64_t need = balance_workspace(parts, E);
     if (need > 0 && (!workspace || !ck_aligned16(workspace) || workspace_bytes < need)) return CK_ERR_WORKSPACE;
     BalanceArgs a;
     a.logits = logits;
@@ -437,10 +514,11 @@ extern "C" int ck_moe_balance_loss_forward(const void* logits, int64_t ld, const
     a.parts = parts;
     a.per_block = ck_ceil_div(tokens, parts);
     a.prob = (float*)workspace;
-    a.count = (int*)workspace + parts * E;
-    a.z = (float*)workspace + 2 * parts * E;
-    a.n = (int*)workspace + 2 * parts * E + parts;
-    a.out = {balance, z, counts, stats};
+    const int64_t cells = parts * balance_padded(E);
+    a.count = (int*)workspace + cells;
+    a.z = (float*)workspace + 2 * cells;
+    a.n = (int*)workspace + 2 * cells + parts;
+    a.out = {balance, z, shares, counts};
     hipStream_t s = (hipStream_t)stream;
     const bool vec = E % ck::kPiece == 0 && ld % ck::kPiece == 0 && ck_aligned16(logits);
     CK_DISPATCH_DTYPE(dtype, {
@@ -450,23 +528,23 @@ extern "C" int ck_moe_balance_loss_forward(const void* logits, int64_t ld, const
         });
     });
     if (parts > 1) {
-        int columns = 1;
-        while (columns < E) columns *= 2;
+        int quads = 1;
+        while (quads * 4 < E) quads *= 2;
         hipLaunchKernelGGL((ck::balance_sum_kernel), dim3(1), dim3(1024), 0, s, a.prob, a.count, a.z, a.n, (int)parts, a.E,
-                           a.k, columns, a.out);
+                           (int)balance_padded(E), a.k, quads, a.out);
     }
     return ck_launch_status();
 }
 
-extern "C" int ck_moe_balance_loss_backward(const void* logits, int64_t ld, const void* mask, const int* counts,
-                                            const int* stats, const float* balance_grad, const float* z_grad, void* d_logits,
-                                            int64_t tokens, int64_t E, int64_t k, int dtype, void* stream) {
-    if (!balance_shape(tokens, E, k) || ld < E) return CK_ERR_SHAPE;
+extern "C" int ck_moe_balance_loss_backward(const void* logits, int64_t ld, const void* mask, const float* shares,
+                                            const float* balance_grad, const float* z_grad, void* d_logits, int64_t tokens,
+                                            int64_t E, int dtype, void* stream) {
+    if (!balance_shape(tokens, E, 1) || ld < E) return CK_ERR_SHAPE;
     if (dtype != CK_F32 && dtype != CK_F16 && dtype != CK_BF16) return CK_ERR_DTYPE;
     if (tokens == 0) return CK_OK;
-    if (!logits || !counts || !stats || !d_logits) return CK_ERR_NULL;
+    if (!logits || !shares || !d_logits) return CK_ERR_NULL;
     if (!ck_aligned_elem(logits, dtype) || !ck_aligned_elem(d_logits, dtype)) return CK_ERR_ALIGN;
-    const BalanceBwd a = {logits, ld, (const uint8_t*)mask, counts, stats, balance_grad, z_grad, d_logits, tokens, (int)E, (int)k};
+    const BalanceBwd a = {logits, ld, (const uint8_t*)mask, shares, balance_grad, z_grad, d_logits, tokens, (int)E};
     hipStream_t s = (hipStream_t)stream;
     const bool vec = E % ck::kPiece == 0 && ld % ck::kPiece == 0 && ck_aligned16(logits) && ck_aligned16(d_logits);
     CK_DISPATCH_DTYPE(dtype, {

@@ -88,7 +88,7 @@ _SIGNATURES = {
         _i32,
         [_p, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i32, _p],
     ),
-    "ck_moe_balance_loss_backward": (_i32, [_p, _i64, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i32, _p]),
+    "ck_moe_balance_loss_backward": (_i32, [_p, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i32, _p]),
     "ck_mx8_quantize": (_i32, [_p, _p, _p, _i64, _i64, _i32, _p]),
     "ck_mx8_dequantize": (_i32, [_p, _p, _p, _i64, _i64, _p, _i64, _i64, _i32, _p]),
     "ck_swiglu_forward_mx8": (_i32, [_p, _p, _i64, _p, _p, _p, _i64, _p, _p, _i64, _i64, _i64, _i32, _p]),
@@ -879,7 +879,7 @@ def moe_balance_loss_workspace_size(tokens: int, E: int) -> int:
     return load_library().ck_moe_balance_loss_workspace_size(tokens, E)
 
 
-def _balance_operands(what: str, logits, mask, counts, stats) -> tuple[int, int, int]:
+def _balance_operands(what: str, logits, mask, shares) -> tuple[int, int, int]:
     """(tokens, experts, distance of the logits' rows)"""
     T, E = logits.shape
     row, column = logits.stride()
@@ -887,43 +887,44 @@ def _balance_operands(what: str, logits, mask, counts, stats) -> tuple[int, int,
         raise ValueError(f"{what}: logits need unit stride over the experts")
     if mask is not None and (mask.numel() != T or mask.dtype != torch.bool or not mask.is_contiguous()):
         raise ValueError(f"{what}: the mask is one dense bool per token")
-    for t, n in ((counts, E), (stats, 2)):
-        if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
-            raise ValueError(f"{what}: counts are dense int32 [experts], stats dense int32 [2]")
+    if shares.dtype != torch.float32 or shares.numel() != E + 1 or not shares.is_contiguous():
+        raise ValueError(f"{what}: shares are dense float32 [experts + 1]")
     return T, E, row if T > 1 else E
 
 
-def moe_balance_loss_forward(logits, selected, mask, balance, z, counts, stats, workspace) -> None:
-    """logits [T, E], selected int64 [T, k], mask [T] or None -> balance, z (fp32 scalars), counts [E], stats [2]."""
+def moe_balance_loss_forward(logits, selected, mask, balance, z, counts, shares, workspace) -> None:
+    """logits [T, E], selected int64 [T, k], mask [T] or None -> balance, z (fp32 scalars), counts [E], shares [E + 1]."""
     lib = load_library()
-    T, E, row = _balance_operands("moe_balance_loss_forward", logits, mask, counts, stats)
+    T, E, row = _balance_operands("moe_balance_loss_forward", logits, mask, shares)
     if selected.dtype != torch.int64 or selected.dim() != 2 or selected.size(0) != T or not selected.is_contiguous():
         raise ValueError("moe_balance_loss_forward: selected must be dense int64 [tokens, k]")
     if balance.dtype != torch.float32 or z.dtype != torch.float32 or balance.numel() != 1 or z.numel() != 1:
         raise ValueError("moe_balance_loss_forward: the losses are one float32 each")
-    with _Launch(logits, selected, mask, balance, z, counts, stats, workspace) as L:
+    if counts.dtype != torch.int32 or counts.numel() != E or not counts.is_contiguous():
+        raise ValueError("moe_balance_loss_forward: counts are dense int32 [experts]")
+    with _Launch(logits, selected, mask, balance, z, counts, shares, workspace) as L:
         _check(
             lib.ck_moe_balance_loss_forward(
-                _ptr(logits), row, _ptr(selected), _ptr(mask), _ptr(balance), _ptr(z), _ptr(counts), _ptr(stats),
+                _ptr(logits), row, _ptr(selected), _ptr(mask), _ptr(balance), _ptr(z), _ptr(counts), _ptr(shares),
                 _ptr(workspace), 0 if workspace is None else workspace.numel(), T, E, selected.size(1),
                 dtype_code(logits.dtype), L.stream),
             "ck_moe_balance_loss_forward",
         )
 
 
-def moe_balance_loss_backward(logits, mask, counts, stats, balance_grad, z_grad, d_logits, top_k: int) -> None:
+def moe_balance_loss_backward(logits, mask, shares, balance_grad, z_grad, d_logits) -> None:
     lib = load_library()
-    T, E, row = _balance_operands("moe_balance_loss_backward", logits, mask, counts, stats)
+    T, E, row = _balance_operands("moe_balance_loss_backward", logits, mask, shares)
     if d_logits.dtype != logits.dtype or d_logits.shape != logits.shape or not d_logits.is_contiguous():
         raise ValueError("moe_balance_loss_backward: d_logits must be dense [tokens, experts] of the logits' dtype")
     for t in (balance_grad, z_grad):
         if t is not None and (t.dtype != torch.float32 or t.numel() != 1):
             raise ValueError("moe_balance_loss_backward: the losses' gradients are one float32 each")
-    with _Launch(logits, mask, counts, stats, balance_grad, z_grad, d_logits) as L:
+    with _Launch(logits, mask, shares, balance_grad, z_grad, d_logits) as L:
         _check(
             lib.ck_moe_balance_loss_backward(
-                _ptr(logits), row, _ptr(mask), _ptr(counts), _ptr(stats), _ptr(balance_grad), _ptr(z_grad),
-                _ptr(d_logits), T, E, top_k, dtype_code(logits.dtype), L.stream),
+                _ptr(logits), row, _ptr(mask), _ptr(shares), _ptr(balance_grad), _ptr(z_grad), _ptr(d_logits), T, E,
+                dtype_code(logits.dtype), L.stream),
             "ck_moe_balance_loss_backward",
         )
 

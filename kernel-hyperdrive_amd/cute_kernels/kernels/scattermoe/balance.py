@@ -35,7 +35,7 @@ def moe_balance_loss_torch(
     return balance, alive.logsumexp(dim=-1).square().sum() / n, counts
 
 
-@cute_op(f"{LIBRARY_NAME}::moe_balance_loss_forward_hip", mutates_args={"balance", "z", "counts", "stats"})
+@cute_op(f"{LIBRARY_NAME}::moe_balance_loss_forward_hip", mutates_args={"balance", "z", "counts", "shares"})
 def moe_balance_loss_forward_hip(
     logits: torch.Tensor,
     selected: torch.Tensor,
@@ -43,25 +43,23 @@ def moe_balance_loss_forward_hip(
     balance: torch.Tensor,
     z: torch.Tensor,
     counts: torch.Tensor,
-    stats: torch.Tensor,
+    shares: torch.Tensor,
 ) -> None:
     nbytes = _C.moe_balance_loss_workspace_size(logits.size(0), logits.size(1))
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes > 0 else None
-    _C.moe_balance_loss_forward(logits, selected, mask, balance, z, counts, stats, workspace)
+    _C.moe_balance_loss_forward(logits, selected, mask, balance, z, counts, shares, workspace)
 
 
 @cute_op(f"{LIBRARY_NAME}::moe_balance_loss_backward_hip", mutates_args={"d_logits"})
 def moe_balance_loss_backward_hip(
     logits: torch.Tensor,
     mask: torch.Tensor | None,
-    counts: torch.Tensor,
-    stats: torch.Tensor,
+    shares: torch.Tensor,
     balance_grad: torch.Tensor | None,
     z_grad: torch.Tensor | None,
     d_logits: torch.Tensor,
-    top_k: int,
 ) -> None:
-    _C.moe_balance_loss_backward(logits, mask, counts, stats, balance_grad, z_grad, d_logits, top_k)
+    _C.moe_balance_loss_backward(logits, mask, shares, balance_grad, z_grad, d_logits)
 
 
 class _MoEBalanceLoss_Cute(torch.autograd.Function):
@@ -71,21 +69,20 @@ class _MoEBalanceLoss_Cute(torch.autograd.Function):
         balance = torch.empty((), dtype=torch.float32, device=device)
         z = torch.empty((), dtype=torch.float32, device=device)
         counts = torch.empty(logits.size(1), dtype=torch.int32, device=device)
-        stats = torch.empty(2, dtype=torch.int32, device=device)
-        moe_balance_loss_forward_hip(logits, selected, mask, balance, z, counts, stats)
-        ctx.save_for_backward(logits, mask, counts, stats)
-        ctx.top_k = selected.size(1)
+        shares = torch.empty(logits.size(1) + 1, dtype=torch.float32, device=device)
+        moe_balance_loss_forward_hip(logits, selected, mask, balance, z, counts, shares)
+        ctx.save_for_backward(logits, mask, shares)
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)
         return balance, z, counts
 
     @staticmethod
     def backward(ctx, balance_grad, z_grad, _counts_grad):
-        logits, mask, counts, stats = ctx.saved_tensors
+        logits, mask, shares = ctx.saved_tensors
         if balance_grad is None and z_grad is None:
             return None, None, None
         d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        moe_balance_loss_backward_hip(logits, mask, counts, stats, balance_grad, z_grad, d_logits, ctx.top_k)
+        moe_balance_loss_backward_hip(logits, mask, shares, balance_grad, z_grad, d_logits)
         return d_logits, None, None
 
 

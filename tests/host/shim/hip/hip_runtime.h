@@ -58,6 +58,9 @@ hipError_t hipGetSymbolAddress(void** address, Symbol& symbol) {
 struct float4 {
     float x, y, z, w;
 };
+struct int4 {
+    int x, y, z, w;
+};
 inline float4 make_float4(float x, float y, float z, float w) { return float4{x, y, z, w}; }
 
 namespace emu {
@@ -313,10 +316,12 @@ inline int emu_readfirstlane(int v) {
 }
 #define __builtin_amdgcn_readfirstlane(v) emu_readfirstlane(v)
 // v_mov_b32 with the DPP controls the kernels use - quad_perm (0 .. 0xFF): lane l reads lane 4 (l / 4) + (ctrl >> 2 (l % 4)) % 4;
-// row_half_mirror (0x141): lane l reads lane 8 (l / 8) + 7 - l % 8
+// row_half_mirror (0x141): lane l reads lane 8 (l / 8) + 7 - l % 8; row_mirror (0x140): lane 16 (l / 16) + 15 - l % 16
 inline int emu_mov_dpp(int v, int ctrl) {
     const int me = __lane_id();
-    const int from = ctrl == 0x141 ? me / 8 * 8 + 7 - me % 8 : me / 4 * 4 + ((ctrl >> (2 * (me % 4))) & 3);
+    const int from = ctrl == 0x141   ? me / 8 * 8 + 7 - me % 8
+                     : ctrl == 0x140 ? me / 16 * 16 + 15 - me % 16
+                                     : me / 4 * 4 + ((ctrl >> (2 * (me % 4))) & 3);
     return emu::wave_instruction(v, [from](auto lane) { return lane(from); });
 }
 #define __builtin_amdgcn_mov_dpp(v, ctrl, row_mask, bank_mask, bound_ctrl) emu_mov_dpp(v, ctrl)
@@ -333,6 +338,7 @@ inline void __threadfence() {}
 #define __builtin_amdgcn_s_waitcnt(code) emu_nothing()
 #define __builtin_amdgcn_s_setprio(level) emu_nothing()
 #define __builtin_amdgcn_rcpf(x) (1.0f / (x))
+#define __builtin_amdgcn_exp2f(x) std::exp2(x)
 
 // ---- gfx950 wave-wide instructions, modelled by their lane layouts -------------------------------------------------------
 // v_mfma_f32_16x16x32: lane l holds A[i = l % 16][k = 8 (l / 16) .. + 7], B[k = 8 (l / 16) .. + 7][j = l % 16] and
