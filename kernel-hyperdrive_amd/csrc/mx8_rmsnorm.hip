@@ -10,6 +10,10 @@
 
 namespace ck {
 
+template <int V>
+struct Int {
+    static constexpr int value = V;
+};
 
 // The backward's launch: workgroups a compute unit holds, and rows a team has in flight, by element size and team width.
 // Measured at 16384 x 4096 bf16 (and 8192 x 4096 fp32): three workgroups with one row in flight 69.1 us, two rows 69.4, three
@@ -21,11 +25,28 @@ constexpr int mx_bwd_residency(int bytes, int tpr) {
 }
 constexpr int mx_bwd_depth(int bytes, int tpr) { return bytes == 4 && tpr < 1024 ? 2 : 1; }
 
+// Sum over the wave, in all lanes: register exchanges up to sixteen lanes (quad_perm 1 0 3 2 and 2 3 0 1, then the mirror
+// images of eight and sixteen, the quads and eights being uniform by then), scalar reads of the four sixteens.  A chain of
+// shuffles is six trips through the LDS unit, which every row waits for (backward of 16384 x 4096 bf16 69.7 -> 68.6 us).
+__device__ __forceinline__ float mx_wave_sum(float v) {
+    auto moved = [](float f, auto ctrl) __attribute__((always_inline)) {
+        return mx_float((uint32_t)__builtin_amdgcn_mov_dpp((int)mx_bits(f), decltype(ctrl)::value, 0xF, 0xF, true));
+    };
+    v += moved(v, Int<0xB1>());
+    v += moved(v, Int<0x4E>());
+    v += moved(v, Int<0x141>());
+    v += moved(v, Int<0x140>());
+    auto lane = [&](int l) __attribute__((always_inline)) {
+        return mx_float((uint32_t)__builtin_amdgcn_readlane((int)mx_bits(v), l));
+    };
+    return (lane(0) + lane(16)) + (lane(32) + lane(48));
+}
+
 // sum over the TPR lanes of a team, in all of them.  Teams wider than a wave meet at one barrier (every thread of the
 // workgroup comes here); `red` holds a float per wave, and two uses in a row take different ones.
 template <int TPR>
 __device__ __forceinline__ float mx_team_sum(float v, float* red) {
-    v = wave_sum(v);
+    v = mx_wave_sum(v);
     if (TPR > CK_WAVE) {
         const int wave = threadIdx.x / CK_WAVE;
         if (lane_id() == 0) red[wave] = v;
@@ -120,7 +141,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
     }
 }
 
-// Rows are dealt round-robin to the teams; a team has the next row in flight while it works on one.
+// Rows are dealt round-robin to the teams.
 // With q the codes and e the step of a block:  dx = r (dy w) - (r^3 mean(dy w s^) e) q,  dw += (dy e r) q  - the steps are
 // folded into factors of a piece, so the kept row costs one conversion an element and no multiplication of its own.
 template <typename T, int TPR, int UNITS, bool HAS_W, bool DSUM, bool VEC>

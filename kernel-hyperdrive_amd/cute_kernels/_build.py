@@ -18,9 +18,12 @@ PACKAGE_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC_DIR = os.path.normpath(os.path.join(PACKAGE_DIR, "..", "csrc"))
 LIB_DIR = os.path.join(PACKAGE_DIR, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libcute_hip.so")
+# the compiled host path (csrc/autograd.cpp), a Python extension module against torch's C++ headers
+AUTOGRAD_SOURCE = os.path.join(CSRC_DIR, "autograd.cpp")
+AUTOGRAD_PATH = os.path.join(LIB_DIR, "cute_autograd.so")
 
-SOURCES = ["status.hip", "add.hip", "swiglu.hip", "rmsnorm.hip", "embedding.hip", "moe_sort.hip", "moe_combine.hip", "expert_bias.hip", "router.hip", "moe_balance.hip",
-           "mx8.hip", "mx8_rmsnorm.hip", "grouped_gemm.hip"]
+SOURCES = ["status.hip", "add.hip", "swiglu.hip", "rmsnorm.hip", "embedding.hip", "moe_sort.hip", "moe_combine.hip",
+           "expert_bias.hip", "router.hip", "moe_balance.hip", "mx8.hip", "mx8_rmsnorm.hip", "grouped_gemm.hip"]
 
 # -packed-fp32-ops off: the packed fp32 VALU forms are not wanted in any kernel of this library
 HIPCC_FLAGS = [
@@ -57,15 +60,44 @@ def _compile(hipcc: str, source: str, obj_dir: str, verbose: bool) -> str:
     return obj
 
 
+def build_autograd(verbose: bool = False) -> str:
+    """Compile the host path with the host compiler (no device code in it); returns its path."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    os.makedirs(LIB_DIR, exist_ok=True)
+    compiler = shutil.which("g++") or shutil.which("c++")
+    if compiler is None:
+        raise RuntimeError("no host C++ compiler: the host path of cute_kernels cannot be built")
+    tmp = AUTOGRAD_PATH + ".tmp"
+    cmd = [compiler, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           "-DTORCH_EXTENSION_NAME=cute_autograd", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    cmd += [f"-I{path}" for path in include_paths("cuda")] + [f"-I{sysconfig.get_paths()['include']}"]
+    cmd += [AUTOGRAD_SOURCE, "-o", tmp]
+    cmd += [f"-L{path}" for path in library_paths("cuda")]
+    cmd += ["-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-lc10_hip", "-ltorch_hip"]
+    result = subprocess.run(cmd, capture_output=True, text=True)
+    if result.returncode != 0:
+        raise RuntimeError(f"building cute_autograd.so failed:\n{result.stderr}")
+    if verbose and result.stderr.strip():
+        print(result.stderr)
+    os.replace(tmp, AUTOGRAD_PATH)
+    return AUTOGRAD_PATH
+
+
 def build(verbose: bool = False, jobs: int | None = None) -> str:
-    """Compile every source and link the shared library; returns its path."""
+    """Compile every source and link the shared library, and the host path beside it; returns the library's path."""
     hipcc = find_hipcc()
     obj_dir = os.path.join(PACKAGE_DIR, "..", "build", "obj")
     os.makedirs(obj_dir, exist_ok=True)
     os.makedirs(LIB_DIR, exist_ok=True)
     jobs = jobs or min(len(SOURCES), os.cpu_count() or 1, 16)
     with ThreadPoolExecutor(max_workers=jobs) as pool:
+        autograd = pool.submit(build_autograd, verbose)
         objects = list(pool.map(lambda src: _compile(hipcc, src, obj_dir, verbose), SOURCES))
+        autograd.result()
     tmp = LIB_PATH + ".tmp"
     link = subprocess.run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", *objects, "-o", tmp],
                           capture_output=True, text=True)

@@ -1,0 +1,49 @@
+"""The compiled host path (``csrc/autograd.cpp``): C++ autograd functions over the library's C entry points, for the operators
+whose calls are short enough for Python's share to show.  The reference's counterpart are the pybind modules of its
+``cpp_jit`` (cute_kernels/jit.py:63-89).
+
+``functions_for(tensor)`` is the module for an eager call on a GPU tensor and None otherwise: while a graph is traced the
+Python autograd functions with their ``cute::`` custom ops are used, and tensors elsewhere get their refusal there."""
+
+from __future__ import annotations
+
+import importlib.util
+import os
+import threading
+
+import torch
+
+from . import _C
+from .utils.custom_op import is_cute_tracing
+
+
+_MODULE = "cute_autograd"
+_module = None
+_lock = threading.Lock()
+
+
+def load():
+    """Import (building first if nothing is built) and connect it to the kernel library; errors are not hidden."""
+    global _module
+    if _module is not None:
+        return _module
+    with _lock:
+        if _module is not None:
+            return _module
+        from . import _build
+
+        if not os.path.exists(_build.AUTOGRAD_PATH):
+            _build.build_autograd()
+        _C.load_library()
+        spec = importlib.util.spec_from_file_location(_MODULE, _build.AUTOGRAD_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.load(_C.library_path(), _C._ABI_VERSION)
+        _module = module
+    return _module
+
+
+def functions_for(tensor: torch.Tensor):
+    if not tensor.is_cuda or torch.compiler.is_compiling() or is_cute_tracing():
+        return None
+    return _module or load()

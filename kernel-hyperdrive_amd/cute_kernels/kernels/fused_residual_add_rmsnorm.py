@@ -11,7 +11,7 @@ one after the other: the sum is rounded to the storage type before it is normali
 import torch
 import torch.nn.functional as F
 
-from .. import _C
+from .. import _C, _native
 from ..constants import LIBRARY_NAME
 from ..cutotune import CutoTuneParameter
 from ..enums import KernelBackend
@@ -132,7 +132,7 @@ class _FusedResidualAddRMSNormMX8_Cute(torch.autograd.Function):
 
     @staticmethod
     def forward(
-        ctx, x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None, eps: float | None
+        ctx, x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None, eps: float
     ) -> tuple[torch.Tensor, torch.Tensor]:
         output, residual_output, saved = rmsnorm_forward_mx8(
             x.contiguous(), residual.contiguous(), None if weight is None else weight.contiguous(), eps
@@ -166,6 +166,11 @@ def fused_residual_add_rmsnorm_cute(
     if checkpoint_8bit and _keeps_8bit(x, weight, memory_efficient, residual):
         assert x.shape == residual.shape, "tensors x and residual should have same shape"
         assert x.dtype == residual.dtype, "tensors x and residual should have same dtype"
+        if eps is None:
+            eps = torch.finfo(x.dtype).eps
+        functions = _native.functions_for(x)
+        if functions is not None:
+            return functions.residual_rmsnorm(x, residual, weight, eps)
         return _FusedResidualAddRMSNormMX8_Cute.apply(x, residual, weight, eps)
     return _FusedResidualAddRMSNorm_Cute.apply(
         x, residual, weight, eps, memory_efficient, kernel_backend_forward, kernel_backend_backward

@@ -16,7 +16,7 @@ The reference has no counterpart; its nearest relative is ``memory_efficient`` o
 
 import torch
 
-from .. import _C
+from .. import _C, _native
 from ..constants import LIBRARY_NAME
 from ..utils import cute_op
 
@@ -81,22 +81,26 @@ def mx8_dequantize_hip(
     _C.mx8_dequantize(codes, scales, output, index, fan)
 
 
-@torch.no_grad()
 def mx8_quantize_cute(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """``(codes, scales)``: int8 of x's shape, and uint8 ``[..., ceil(H / 32)]``.  float32, float16 or bfloat16; not
     differentiable (a checkpoint is read in a backward, not differentiated through)."""
+    functions = _native.functions_for(x)
+    if functions is not None:
+        return functions.mx8_quantize(x)
     if x.dim() == 0:
         raise ValueError("mx8_quantize_cute: x needs at least one dimension")
-    rows = x.unsqueeze(0) if x.dim() == 1 else x
+    rows = x.detach().unsqueeze(0) if x.dim() == 1 else x.detach()
     rows = rows.contiguous()
     codes, scales = new_mx8(rows.shape, x.device)
     mx8_quantize_hip(rows, codes, scales)
     return (codes.squeeze(0), scales.squeeze(0)) if x.dim() == 1 else (codes, scales)
 
 
-@torch.no_grad()
 def mx8_dequantize_cute(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     """The values ``(codes, scales)`` stand for, exact in ``dtype`` (beyond float16's range: its largest finite number)."""
+    functions = _native.functions_for(codes)
+    if functions is not None:
+        return functions.mx8_dequantize(codes, scales, dtype)
     if codes.dim() == 0:
         raise ValueError("mx8_dequantize_cute: codes need at least one dimension")
     is_1d = codes.dim() == 1

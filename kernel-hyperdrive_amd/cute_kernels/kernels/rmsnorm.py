@@ -13,7 +13,7 @@ call compatibility: a row is always held whole.
 import torch
 import torch.nn.functional as F
 
-from .. import _C
+from .. import _C, _native
 from ..constants import LIBRARY_NAME, MAX_ROW_LENGTH
 from ..cutotune import CutoTuneConfig, CutoTuneParameter, cutotune, get_cartesian_product_cutotune_configs
 from ..enums import KernelBackend
@@ -284,8 +284,6 @@ def _keeps_8bit(x: torch.Tensor, weight: torch.Tensor | None, memory_efficient: 
 
 def rmsnorm_forward_mx8(x, residual, weight, eps):
     """(output, x + residual or None, what the backward needs) of contiguous operands."""
-    if eps is None:
-        eps = torch.finfo(x.dtype).eps
     output = torch.empty_like(x)
     residual_output = None if residual is None else torch.empty_like(x)
     H = x.size(-1)
@@ -310,7 +308,7 @@ class _RMSNormMX8_Cute(torch.autograd.Function):
     """As ``_RMSNorm_Cute``, with x saved in 8 bits (see mx8.py) by the forward's own pass; 1 / rms is saved as well."""
 
     @staticmethod
-    def forward(ctx, x: torch.Tensor, weight: torch.Tensor | None, eps: float | None) -> torch.Tensor:
+    def forward(ctx, x: torch.Tensor, weight: torch.Tensor | None, eps: float) -> torch.Tensor:
         output, _, saved = rmsnorm_forward_mx8(x.contiguous(), None, None if weight is None else weight.contiguous(), eps)
         ctx.save_for_backward(*saved)
         return output
@@ -337,7 +335,10 @@ def rmsnorm_cute(
     """``checkpoint_8bit``: keep x for the backward in 8 bits (see mx8.py); the output is that of the exact rows, the gradients
     are those at the kept rows with the exact rows' 1 / rms.  Not with ``memory_efficient``; the tunables have no meaning there."""
     if checkpoint_8bit and _keeps_8bit(x, weight, memory_efficient):
-        return _RMSNormMX8_Cute.apply(x, weight, eps)
+        if eps is None:
+            eps = torch.finfo(x.dtype).eps
+        functions = _native.functions_for(x)
+        return _RMSNormMX8_Cute.apply(x, weight, eps) if functions is None else functions.rmsnorm(x, weight, eps)
     return _RMSNorm_Cute.apply(
         x,
         weight,

@@ -12,7 +12,7 @@ Gradients reach the logits through p and lse; the counts are whole numbers and h
 
 import torch
 
-from ... import _C
+from ... import _C, _native
 from ...constants import LIBRARY_NAME
 from ...utils import cute_op
 
@@ -125,4 +125,7 @@ def moe_balance_loss_cute(
         if token_mask.dtype != torch.bool or token_mask.shape != router_logits.shape[:-1]:
             raise ValueError("moe_balance_loss_cute: token_mask is one bool per token")
         token_mask = token_mask.reshape(-1).contiguous()
-    return _MoEBalanceLoss_Cute.apply(logits, selected_experts, token_mask)
+    functions = _native.functions_for(logits)
+    if functions is None:
+        return _MoEBalanceLoss_Cute.apply(logits, selected_experts, token_mask)
+    return functions.moe_balance_loss(logits, selected_experts, token_mask)

@@ -8,7 +8,7 @@ backend whose only tunable is the workgroup size.
 import torch
 import torch.nn.functional as F
 
-from .. import _C
+from .. import _C, _native
 from ..constants import COMMON_WORKGROUP_SIZES, LIBRARY_NAME
 from ..cutotune import CutoTuneConfig, CutoTuneParameter, cutotune, get_cartesian_product_cutotune_configs
 from ..enums import KernelBackend
@@ -145,7 +145,8 @@ def swiglu_cute(
     if checkpoint_8bit and torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad):
         assert gate.shape == up.shape, "tensors gate and up should have same shape"
         assert gate.dtype == up.dtype, "tensors gate and up should have same dtype"
-        return _SwigluMX8_Cute.apply(gate, up)
+        functions = _native.functions_for(gate)
+        return _SwigluMX8_Cute.apply(gate, up) if functions is None else functions.swiglu(gate, up)
     return _Swiglu_Cute.apply(
         gate, up, kernel_backend_forward, kernel_backend_backward, BLOCK_SIZE_forward, BLOCK_SIZE_backward
     )

@@ -8,7 +8,7 @@ The reference tunes a 2-D (BLOCK_SIZE_B, BLOCK_SIZE_H) Triton tile; the HIP kern
 import torch
 import torch.nn.functional as F
 
-from .. import _C
+from .. import _C, _native
 from ..constants import COMMON_WORKGROUP_SIZES, LIBRARY_NAME
 from ..cutotune import CutoTuneConfig, CutoTuneParameter, cutotune, get_cartesian_product_cutotune_configs
 from ..enums import KernelBackend
@@ -104,7 +104,7 @@ def swiglu_unchunked_forward_mx8_hip(x: torch.Tensor, output: torch.Tensor, kept
 
 @cute_op(f"{LIBRARY_NAME}::swiglu_unchunked_backward_mx8_hip", mutates_args={"x_grad", "activation"})
 def swiglu_unchunked_backward_mx8_hip(
-    kept: torch.Tensor, output_grad: torch.Tensor, x_grad: torch.Tensor, activation: torch.Tensor | None = None
+    kept: torch.Tensor, output_grad: torch.Tensor, x_grad: torch.Tensor, activation: torch.Tensor | None
 ) -> None:
     """``activation``: also written, with the forward's output at the kept inputs."""
     _C.swiglu_unchunked_backward_mx8(kept, output_grad, x_grad, activation)
@@ -129,7 +129,7 @@ class _SwigluUnchunkedMX8_Cute(torch.autograd.Function):
         output_grad = output_grad.contiguous()
         *lead, h = output_grad.shape
         x_grad = torch.empty((*lead, 2 * h), device=output_grad.device, dtype=output_grad.dtype)
-        swiglu_unchunked_backward_mx8_hip(ctx.saved_tensors[0], output_grad, x_grad)
+        swiglu_unchunked_backward_mx8_hip(ctx.saved_tensors[0], output_grad, x_grad, None)
         return x_grad
 
 
@@ -146,7 +146,8 @@ def swiglu_unchunked_cute(
     """``checkpoint_8bit``: keep x for the backward in 8 bits (see mx8.py); the output is that of the exact x, the gradient
     that at the kept values.  The other tunables have no meaning there."""
     if checkpoint_8bit and torch.is_grad_enabled() and x.requires_grad:
-        return _SwigluUnchunkedMX8_Cute.apply(x)
+        functions = _native.functions_for(x)
+        return _SwigluUnchunkedMX8_Cute.apply(x) if functions is None else functions.swiglu_unchunked(x)
     return _SwigluUnchunked_Cute.apply(
         x,
         kernel_backend_forward,

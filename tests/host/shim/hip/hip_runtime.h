@@ -315,6 +315,10 @@ inline int emu_readfirstlane(int v) {
     return emu::wave_instruction(v, [](auto lane) { return lane(0); });
 }
 #define __builtin_amdgcn_readfirstlane(v) emu_readfirstlane(v)
+inline int emu_readlane(int v, int from) {
+    return emu::wave_instruction(v, [from](auto lane) { return lane(from); });
+}
+#define __builtin_amdgcn_readlane(v, from) emu_readlane(v, from)
 // v_mov_b32 with the DPP controls the kernels use - quad_perm (0 .. 0xFF): lane l reads lane 4 (l / 4) + (ctrl >> 2 (l % 4)) % 4;
 // row_half_mirror (0x141): lane l reads lane 8 (l / 8) + 7 - l % 8; row_mirror (0x140): lane 16 (l / 16) + 15 - l % 16
 inline int emu_mov_dpp(int v, int ctrl) {

@@ -638,3 +638,59 @@ def test_results_repeat_bit_for_bit(gpu):
     first = _step(gpu, leaves, dy)
     for _ in range(2):
         assert all(torch.equal(a, b) for a, b in zip(first, _step(gpu, leaves, dy)))
+
+
+def _every_operator(gpu, dtype):
+    """All results and gradients of the operators with an 8-bit checkpoint, the pair and the balance loss."""
+    import cute_kernels as ck
+
+    out = []
+    x, res = randn((37, 200), dtype, 401).to(gpu).requires_grad_(True), randn((37, 200), dtype, 402).to(gpu).requires_grad_(True)
+    w = randn((200,), dtype, 403, 0.1, 1.0).to(gpu).requires_grad_(True)
+    dy = randn((37, 200), dtype, 404).to(gpu)
+    for weight in (w, None):
+        leaves = (x, w) if weight is not None else (x,)
+        y = ck.rmsnorm_cute(x, weight, None, checkpoint_8bit=True)
+        out += [y, *torch.autograd.grad(y, leaves, dy)]
+        y, s = ck.fused_residual_add_rmsnorm_cute(x, res, weight, 1e-6, checkpoint_8bit=True)
+        out += [y, s, *torch.autograd.grad((y, s), (*leaves, res), (dy, dy))]
+    y = ck.swiglu_cute(x.t(), res.t(), checkpoint_8bit=True)
+    out += [y, *torch.autograd.grad(y, (x, res), dy.t())]
+    y = ck.swiglu_unchunked_cute(x, checkpoint_8bit=True)
+    out += [y, *torch.autograd.grad(y, x, dy[:, :100])]
+    y = ck.swiglu_unchunked_cute(x[3], checkpoint_8bit=True)
+    out += [y, *torch.autograd.grad(y, x, dy[3, :100])]
+    codes, scales = ck.mx8_quantize_cute(x)
+    out += [codes, scales, ck.mx8_dequantize_cute(codes, scales, dtype), *ck.mx8_quantize_cute(x[0])]
+    ids = x.detach().float().topk(3, dim=-1).indices
+    mask = (torch.arange(37) % 5 != 0).to(gpu)
+    for chosen in (ids, None):
+        balance, z, counts = ck.moe_balance_loss_cute(x, chosen, mask, top_k=3)
+        out += [balance, z, counts, *torch.autograd.grad(2 * balance + z, x)]
+    return [t.detach() for t in out]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_compiled_and_python_host_paths_agree(gpu, dtype, monkeypatch):
+    """Eager calls on GPU tensors go through csrc/autograd.cpp, traced ones through the Python autograd functions and their
+    custom ops: the same kernels on the same buffers, bit for bit."""
+    from cute_kernels import _native
+    from cute_kernels.utils import set_cute_tracing
+
+    announce("host paths", dtype)
+    if gpu.type == "cuda":
+        assert _native.functions_for(torch.zeros(1, device=gpu)) is not None
+    eager = _every_operator(gpu, dtype)
+    if gpu.type == "cuda":
+        monkeypatch.setattr(_native, "functions_for", lambda tensor: None)
+        python = _every_operator(gpu, dtype)
+        assert all(torch.equal(a, b) for a, b in zip(eager, python))
+        monkeypatch.undo()
+        assert _native.functions_for(torch.zeros(1, device=gpu)) is not None
+    set_cute_tracing(True)
+    try:
+        assert _native.functions_for(torch.zeros(1, device=gpu)) is None
+        traced = _every_operator(gpu, dtype)
+    finally:
+        set_cute_tracing(False)
+    assert len(traced) == len(eager) and all(torch.equal(a, b) for a, b in zip(eager, traced))
