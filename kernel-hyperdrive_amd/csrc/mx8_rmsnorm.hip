@@ -508,7 +508,7 @@ extern "C" int ck_rmsnorm_backward_mx8(const void* codes, const void* scales, co
     if (B < 0 || H < 0 || H > kMxMaxRow) return CK_ERR_SHAPE;
     if (!mx_rows_dtype(dtype)) return CK_ERR_DTYPE;
     hipStream_t s = (hipStream_t)stream;
-    if (H == 0) return CK_OK;
+    if (H == 0 || (B == 0 && !weight)) return CK_OK;
     if (weight && !weight_grad) return CK_ERR_NULL;
     if (weight && (!ck_aligned_elem(weight, dtype) || !ck_aligned_elem(weight_grad, dtype))) return CK_ERR_ALIGN;
     const int padded = (int)(ck::mx_blocks(H) * ck::kMxBlock);

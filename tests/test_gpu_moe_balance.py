@@ -55,6 +55,7 @@ def check(gpu, logits, selected, mask, dtype, g_balance=0.5, g_z=0.25, ids_type=
     want = reference(logits.reshape(-1, E), selected.reshape(-1, k).long(), None if mask is None else mask.reshape(-1),
                      g_balance, g_z)
     assert torch.equal(counts.cpu().long(), want[2])
+    balance, z_loss = balance.detach(), z_loss.detach()
     assert abs(float(balance) - float(want[0])) <= 2.0 ** -19 * float(want[0]) + 1e-30
     assert abs(float(z_loss) - float(want[1])) <= 2.0 ** -19 * float(want[1]) + 1e-30
     assert_rounded(d.reshape(-1, E), want[3], dtype, 2.0 ** -19, want[4], "d_logits")
