@@ -366,8 +366,7 @@ int ck_moe_balance_loss_backward(const void* logits, int64_t ld, const void* mas
  * block with a NaN or an infinity, which stands for NaNs.
  *   codes: H bytes a row, scales: ceil(H / 32) bytes a row (dense unless a stride is passed)
  * ck_mx8_quantize    x [rows, H] -> codes, scales
- * ck_mx8_dequantize  output row r = kept row r, or kept row index[r] / fan (index int64 [rows]; a row outside
- *                    [0, source_rows) becomes zeros).  A value beyond fp16's range becomes its largest finite number.
+ * ck_mx8_dequantize  codes, scales -> output [rows, H].  A value beyond fp16's range becomes its largest finite number.
  * ck_swiglu_forward_mx8 / _backward_mx8
  *                    y = up * gate * sigmoid(gate), with gate and up also written in 8 bits; the gradients from those.
  *                    Rows of gate, up and their gradients are `ldx` elements apart (two tensors, or the halves of one),
@@ -383,8 +382,7 @@ int ck_moe_balance_loss_backward(const void* logits, int64_t ld, const void* mas
  * for RMSNorm.
  * ------------------------------------------------------------------------------------------- */
 int ck_mx8_quantize(const void* x, void* codes, void* scales, int64_t rows, int64_t H, int dtype, void* stream);
-int ck_mx8_dequantize(const void* codes, const void* scales, const int64_t* index, int64_t fan, int64_t source_rows,
-                      void* output, int64_t rows, int64_t H, int dtype, void* stream);
+int ck_mx8_dequantize(const void* codes, const void* scales, void* output, int64_t rows, int64_t H, int dtype, void* stream);
 int ck_swiglu_forward_mx8(const void* gate, const void* up, int64_t ldx, void* output, void* gate_codes, void* up_codes,
                           int64_t ldc, void* gate_scales, void* up_scales, int64_t lds, int64_t rows, int64_t H, int dtype,
                           void* stream);

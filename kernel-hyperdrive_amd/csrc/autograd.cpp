@@ -152,8 +152,7 @@ Tensor mx8_dequantize(const Tensor& input_codes, const Tensor& input_scales, at:
     const int code = dtype_code(dtype);
     const c10::DeviceGuard guard(codes.device());
     Tensor output = at::empty(codes.sizes(), codes.options().dtype(dtype));
-    check(lib.ck_mx8_dequantize(data(codes), data(scales), nullptr, 1, r.count, data(output), r.count, r.H, code,
-                                stream_of(codes)),
+    check(lib.ck_mx8_dequantize(data(codes), data(scales), data(output), r.count, r.H, code, stream_of(codes)),
           "ck_mx8_dequantize");
     return output;
 }

@@ -54,11 +54,9 @@ __device__ __forceinline__ float mx_limit<F16>(float v) {
     return v > 65504.f ? 65504.f : (v < -65504.f ? -65504.f : v);  // (a NaN fails both comparisons)
 }
 
-// out row r is row (index != NULL ? index[r] / fan : r) of the kept matrix; rows outside it become zeros
-template <typename T, int MODE, bool GATHER>
+template <typename T, int MODE>
 __global__ void __launch_bounds__(kMxThreads)
     mx8_dequantize_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                          const int64_t* __restrict__ index, int64_t fan, int64_t source_rows,
                           typename T::storage_t* __restrict__ out, MxShape shape) {
     constexpr int N = kMxPiece<T>, LANES = kMxLanes<T>;
     constexpr bool VEC = MODE != kMxAny;
@@ -73,25 +71,19 @@ __global__ void __launch_bounds__(kMxThreads)
         in[i] = MxCodes<N>{};
         scale[i] = 7;
         if (mx_has<MODE>(shape, p, a)) {
-            const int64_t row = GATHER ? index[a.row] / fan : a.row;
-            if (!GATHER || (row >= 0 && row < source_rows)) {
-                in[i] = load_codes<N, VEC>(codes + row * shape.h + a.col, a.n);
-                scale[i] = scales[row * blocks + a.block];
-            }
+            in[i] = load_codes<N, VEC>(codes + a.row * shape.h + a.col, a.n);
+            scale[i] = scales[a.row * blocks + a.block];
         }
     }
 #pragma unroll
     for (int i = 0; i < kMxUnroll; ++i) {
         const uint32_t p = base + i * kMxThreads;
         const MxAt a = mx_at<N, MODE>(shape, p);
-        float v[N];
-        mx_decode(in[i], mx_step(scale[i]), v);
         if (mx_has<MODE>(shape, p, a)) {
+            const float step = mx_step(scale[i]);
             Piece<T, N> o;
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                o.put(j, mx_limit<T>(v[j]));
-            }
+            for (int j = 0; j < N; ++j) o.put(j, mx_limit<T>(mx_code(in[i], j) * step));
             store_piece<T, N, VEC>(o, out + a.row * shape.h + a.col, a.n);
         }
     }
@@ -269,34 +261,23 @@ extern "C" int ck_mx8_quantize(const void* x, void* codes, void* scales, int64_t
     return ck_launch_status();
 }
 
-extern "C" int ck_mx8_dequantize(const void* codes, const void* scales, const int64_t* index, int64_t fan,
-                                 int64_t source_rows, void* output, int64_t rows, int64_t H, int dtype, void* stream) {
-    if (rows < 0 || H < 0 || fan < 1 || source_rows < 0 || (!index && source_rows < rows)) return CK_ERR_SHAPE;
+extern "C" int ck_mx8_dequantize(const void* codes, const void* scales, void* output, int64_t rows, int64_t H, int dtype,
+                                 void* stream) {
+    if (rows < 0 || H < 0) return CK_ERR_SHAPE;
     if (!mx_dtype(dtype)) return CK_ERR_DTYPE;
     if (rows == 0 || H == 0) return CK_OK;
-    if (!output || (source_rows > 0 && (!codes || !scales))) return CK_ERR_NULL;
+    if (!codes || !scales || !output) return CK_ERR_NULL;
     if (!ck_aligned_elem(output, dtype)) return CK_ERR_ALIGN;
     ck::MxShape shape;
     if (!ck::mx_shape(rows, H, mx_piece(dtype), &shape)) return CK_ERR_SHAPE;
     hipStream_t s = (hipStream_t)stream;
-    const int mode = mx_mode(H, mx_piece(dtype), ck_aligned16(output) && aligned8(codes), index == nullptr);
+    const int mode = mx_mode(H, mx_piece(dtype), ck_aligned16(output) && aligned8(codes), true);
     CK_DISPATCH_DTYPE(dtype, {
         typedef typename T::storage_t S;
-        if (index == nullptr) {
-            CK_MX_MODE(mode, {
-                hipLaunchKernelGGL((ck::mx8_dequantize_kernel<T, MODE, false>), mx_grid(shape, ck::kMxUnroll),
-                                   dim3(ck::kMxThreads), 0, s, (const int8_t*)codes, (const uint8_t*)scales, index, fan,
-                                   source_rows, (S*)output, shape);
-            });
-        } else if (mode == ck::kMxRows) {
-            hipLaunchKernelGGL((ck::mx8_dequantize_kernel<T, ck::kMxRows, true>), mx_grid(shape, ck::kMxUnroll),
-                               dim3(ck::kMxThreads), 0, s, (const int8_t*)codes, (const uint8_t*)scales, index, fan,
-                               source_rows, (S*)output, shape);
-        } else {
-            hipLaunchKernelGGL((ck::mx8_dequantize_kernel<T, ck::kMxAny, true>), mx_grid(shape, ck::kMxUnroll),
-                               dim3(ck::kMxThreads), 0, s, (const int8_t*)codes, (const uint8_t*)scales, index, fan,
-                               source_rows, (S*)output, shape);
-        }
+        CK_MX_MODE(mode, {
+            hipLaunchKernelGGL((ck::mx8_dequantize_kernel<T, MODE>), mx_grid(shape, ck::kMxUnroll), dim3(ck::kMxThreads), 0, s,
+                               (const int8_t*)codes, (const uint8_t*)scales, (S*)output, shape);
+        });
     });
     return ck_launch_status();
 }

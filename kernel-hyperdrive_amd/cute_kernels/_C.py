@@ -90,7 +90,7 @@ _SIGNATURES = {
     ),
     "ck_moe_balance_loss_backward": (_i32, [_p, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i32, _p]),
     "ck_mx8_quantize": (_i32, [_p, _p, _p, _i64, _i64, _i32, _p]),
-    "ck_mx8_dequantize": (_i32, [_p, _p, _p, _i64, _i64, _p, _i64, _i64, _i32, _p]),
+    "ck_mx8_dequantize": (_i32, [_p, _p, _p, _i64, _i64, _i32, _p]),
     "ck_swiglu_forward_mx8": (_i32, [_p, _p, _i64, _p, _p, _p, _i64, _p, _p, _i64, _i64, _i64, _i32, _p]),
     "ck_swiglu_backward_mx8": (_i32, [_p, _p, _i64, _p, _p, _i64, _p, _p, _p, _i64, _p, _i64, _i64, _i32, _p]),
     "ck_rmsnorm_forward_mx8": (_i32, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _f32, _i32, _p]),
@@ -974,20 +974,15 @@ def mx8_quantize(x, codes, scales) -> None:
                "ck_mx8_quantize")
 
 
-def mx8_dequantize(codes, scales, output, index=None, fan: int = 1) -> None:
-    """output = the values of (codes, scales); with `index` (int64 [rows of output]) row r comes from row index[r] // fan."""
+def mx8_dequantize(codes, scales, output) -> None:
     lib = load_library()
     _mx8_pair("mx8_dequantize", codes, scales)
     rows, H = _rows_alike("mx8_dequantize", output)
-    source_rows = codes.numel() // H if H > 0 else 0
-    if codes.shape[-1] != H or (index is None and rows != source_rows):
-        raise ValueError("mx8_dequantize: the output has the rows' length, and their number unless an index is given")
-    if index is not None and (index.dtype != torch.int64 or index.numel() != rows or not index.is_contiguous()):
-        raise ValueError("mx8_dequantize: one int64 index per output row")
-    with _Launch(codes, scales, index, output) as L:
+    if codes.shape != output.shape:
+        raise ValueError("mx8_dequantize: one code per element")
+    with _Launch(codes, scales, output) as L:
         _check(
-            lib.ck_mx8_dequantize(_ptr(codes), _ptr(scales), _ptr(index), fan, source_rows, _ptr(output), rows, H,
-                                  dtype_code(output.dtype), L.stream),
+            lib.ck_mx8_dequantize(_ptr(codes), _ptr(scales), _ptr(output), rows, H, dtype_code(output.dtype), L.stream),
             "ck_mx8_dequantize",
         )
 

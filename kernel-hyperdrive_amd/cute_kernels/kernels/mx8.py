@@ -75,10 +75,8 @@ def mx8_quantize_hip(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor)
 
 
 @cute_op(f"{LIBRARY_NAME}::mx8_dequantize_hip", mutates_args={"output"})
-def mx8_dequantize_hip(
-    codes: torch.Tensor, scales: torch.Tensor, output: torch.Tensor, index: torch.Tensor | None = None, fan: int = 1
-) -> None:
-    _C.mx8_dequantize(codes, scales, output, index, fan)
+def mx8_dequantize_hip(codes: torch.Tensor, scales: torch.Tensor, output: torch.Tensor) -> None:
+    _C.mx8_dequantize(codes, scales, output)
 
 
 def mx8_quantize_cute(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:

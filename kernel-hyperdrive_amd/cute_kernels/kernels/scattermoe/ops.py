@@ -31,7 +31,7 @@ from ... import _C
 from ...constants import LIBRARY_NAME
 from ...cutotune import CutoTuneConfig, CutoTuneParameter, cutotune, get_cartesian_product_cutotune_configs
 from ...utils import cute_op
-from ..mx8 import kept_pair, mx8_dequantize_hip, mx8_quantize_hip, new_kept, new_mx8
+from ..mx8 import kept_pair, mx8_quantize_hip, new_kept, new_mx8
 from ..swiglu_unchunked import swiglu_unchunked_backward_mx8_hip
 
 
@@ -516,15 +516,15 @@ class _ScatteredGLUExperts(torch.autograd.Function):
 
 
 class _ScatteredGLUExpertsMX8(torch.autograd.Function):
-    """``_ScatteredGLUExperts`` with what its backward needs - x, c_fc's output and the expert outputs - saved in 8 bits
-    (see mx8.py), and the activation not saved at all but recomputed by the pass that computes h's gradient.  The output
-    does not change; the gradients are those at the kept values."""
+    """``_ScatteredGLUExperts`` with the large part of what its backward needs - c_fc's output and the expert outputs - saved in
+    8 bits (see mx8.py), and the activation not saved at all but recomputed by the pass that computes h's gradient.  (x is
+    saved as it is: the router's backward holds on to it anyway.)  The output does not change; the gradients are those at
+    the kept values."""
 
     @staticmethod
     def forward(ctx, x, w_fc, w_proj, k, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates):
         num_slots = sorted_expert_idxs.size(0)
         half = w_proj.size(1)
-        x = x.contiguous()
         h = torch.empty(num_slots, 2 * half, device=x.device, dtype=x.dtype)
         act = torch.empty(num_slots, half, device=x.device, dtype=x.dtype)
         scatter2scatter_glu(
@@ -558,19 +558,17 @@ class _ScatteredGLUExpertsMX8(torch.autograd.Function):
         moe_combine_forward(expanded=expanded, gates=gates, out=output)
         y_codes, y_scales = new_mx8(expanded.shape, x.device)
         mx8_quantize_hip(expanded, y_codes, y_scales)
-        x_codes, x_scales = new_mx8(x.shape, x.device)
-        mx8_quantize_hip(x, x_codes, x_scales)
         ctx.save_for_backward(
-            w_fc, w_proj, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates, x_codes, x_scales, h_kept,
-            y_codes, y_scales
+            x, w_fc, w_proj, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates, h_kept, y_codes, y_scales
         )
         ctx.k = k
         return output
 
     @staticmethod
     def backward(ctx, grad_out):
-        (w_fc, w_proj, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates, x_codes, x_scales, h_kept,
-         y_codes, y_scales) = ctx.saved_tensors
+        x, w_fc, w_proj, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates, h_kept, y_codes, y_scales = (
+            ctx.saved_tensors
+        )
         k = ctx.k
         E = w_fc.size(0)
         num_slots, half = sorted_expert_idxs.size(0), w_proj.size(1)
@@ -610,8 +608,8 @@ class _ScatteredGLUExpertsMX8(torch.autograd.Function):
         group_bwd_W(DY=grouped_grad_out, X=act, expert_offsets=expert_offsets, DW=d_w_proj, E=E)
         del act, grouped_grad_out
 
-        grouped_x = torch.empty(num_slots, x_codes.size(1), dtype=dtype, device=device)
-        mx8_dequantize_hip(x_codes, x_scales, grouped_x, sorted_scattered_idxs, k)
+        grouped_x = torch.empty(num_slots, x.size(1), dtype=dtype, device=device)
+        group(A=x, sorted_expert_idxs=sorted_scattered_idxs, out=grouped_x, fan_out=k)
         d_w_fc = torch.empty_like(w_fc)
         group_bwd_W(DY=d_h, X=grouped_x, expert_offsets=expert_offsets, DW=d_w_fc, E=E)
         d_expanded_input = grouped_x  # reused once the weight gradient has consumed it
@@ -626,7 +624,7 @@ class _ScatteredGLUExpertsMX8(torch.autograd.Function):
             y_grouped=False,
             expert_offsets=expert_offsets,
         )
-        d_input = _sum_over_slots(d_expanded_input, x_codes.size(0), k)
+        d_input = _sum_over_slots(d_expanded_input, x.size(0), k)
         # x, w_fc, w_proj, k, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates
         return d_input, d_w_fc, d_w_proj, None, None, None, None, d_gates
 
@@ -634,7 +632,7 @@ class _ScatteredGLUExpertsMX8(torch.autograd.Function):
 def scattered_glu_experts(
     inputs, w_fc, w_proj, k, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates, checkpoint_8bit=False
 ):
-    """``checkpoint_8bit``: keep what the backward needs in 8 bits (``_ScatteredGLUExpertsMX8``)."""
+    """``checkpoint_8bit``: keep the intermediate rows the backward needs in 8 bits (``_ScatteredGLUExpertsMX8``)."""
     if checkpoint_8bit and torch.is_grad_enabled() and any(t.requires_grad for t in (inputs, w_fc, w_proj, gates)):
         return _ScatteredGLUExpertsMX8.apply(
             inputs, w_fc, w_proj, k, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates

@@ -160,7 +160,7 @@ def test_fp16_end_of_range(gpu):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_layouts_of_the_pair(gpu, dtype):
-    from cute_kernels import _C, mx8_dequantize_cute, mx8_quantize_cute
+    from cute_kernels import mx8_quantize_cute
 
     announce("mx8 layouts", dtype)
     x = randn((64, 96), dtype, 3)
@@ -174,19 +174,6 @@ def test_layouts_of_the_pair(gpu, dtype):
     codes, scales = mx8_quantize_cute(shifted)
     want = encode64(flat[3:].view(64, 96))
     assert torch.equal(codes.cpu().long(), want[0]) and torch.equal(scales.cpu().long(), want[1])
-    # rows gathered through an index, as the experts read them; rows that do not exist become zeros
-    codes, scales = mx8_quantize_cute(xg)
-    index = torch.tensor([5, 0, 127, 126, 1, 1, -2, 128, 130, 64], device=gpu)
-    for width in (96, 33):
-        part = xg[:, :width].contiguous()
-        codes, scales = mx8_quantize_cute(part)
-        out = torch.full((10, width), 7.0, dtype=dtype, device=gpu)
-        _C.mx8_dequantize(codes, scales, out, index, 2)
-        whole = mx8_dequantize_cute(codes, scales, dtype)
-        rows = [2, 0, 63, 63, 0, 0, None, None, None, 32]
-        for r, source in enumerate(rows):
-            expected = torch.zeros(width, dtype=dtype, device=gpu) if source is None else whole[source]
-            assert torch.equal(out[r], expected), (width, r)
 
 
 # ---- SwiGLU ---------------------------------------------------------------------------------------------------------------
@@ -497,7 +484,6 @@ def test_moe_layer(gpu, dtype, shape):
     rounded = lambda t: t.to(dtype).double()
     w_fc, w_proj = moe.c_fc.weight.detach().cpu().double(), moe.c_proj.weight.detach().cpu().double()
     x64, d64, gates, selected = x.double(), dy.double(), gates.cpu().double(), selected.cpu()
-    kx = kept64(x)
     d_x_rows = torch.zeros(T, k, H, dtype=torch.float64)
     d_fc, d_proj = torch.zeros_like(w_fc), torch.zeros_like(w_proj)
     d_gates = torch.zeros(T, k, dtype=torch.float64)
@@ -513,7 +499,7 @@ def test_moe_layer(gpu, dtype, shape):
         d_act = rounded(grad @ w_proj[e])
         d_h = rounded(torch.cat([d_act * kg * s, d_act * ku * (s + kg * s * (1 - s))], dim=1))
         d_proj[e] = grad.t() @ rounded(ku * kg * s)
-        d_fc[e] = d_h.t() @ kx[t]
+        d_fc[e] = d_h.t() @ x64[t]
         d_x_rows[t, slot] = rounded(d_h @ w_fc[e])
     # the router adds its own gradient to x: softmax over the k logits, then its linear
     router = gates * (d_gates - (gates * d_gates).sum(-1, keepdim=True))
@@ -547,8 +533,8 @@ def test_moe_layer_saves_less(gpu):
     plain, _ = saved(moe)
     moe.checkpoint_8bit = True
     kept, _ = saved(moe)
-    rows = 512 * (2 * 384 + 256) + 256 * 256
-    assert kept < plain - rows  # at the least a byte an element less
+    rows = 512 * (2 * 384 + 256) + 512 * 384
+    assert kept < plain - rows  # a byte an element less (the scale bytes aside), two for the activation
 
 
 def test_moe_layer_refuses_what_it_cannot_keep(gpu):

@@ -33,14 +33,12 @@ def test_pair_argument_checks(lib):  # noqa: F811
     assert f(None, None, None, 0, 64, BF16, None) == OK
     assert f(None, None, None, 4, 0, BF16, None) == OK
     g = lib.ck_mx8_dequantize
-    #        codes scales index fan src out rows H dtype stream
-    assert g(P, P, None, 1, 3, P, 4, 64, BF16, None) == SHAPE  # more rows out than kept, and no index
-    assert g(P, P, P, 0, 3, P, 4, 64, BF16, None) == SHAPE
-    assert g(P, P, P, 1, -1, P, 4, 64, BF16, None) == SHAPE
-    assert g(P, P, P, 1, 3, None, 4, 64, BF16, None) == NULL
-    assert g(None, P, P, 1, 3, P, 4, 64, BF16, None) == NULL
-    assert g(P, P, None, 1, 4, P + 1, 4, 64, F32, None) == ALIGN
-    assert g(P, P, None, 1, 4, P, 4, 64, 3, None) == DTYPE
+    assert g(P, P, P, 4, -64, BF16, None) == SHAPE
+    assert g(P, P, None, 4, 64, BF16, None) == NULL
+    assert g(None, P, P, 4, 64, BF16, None) == NULL
+    assert g(P, P, P + 1, 4, 64, F32, None) == ALIGN
+    assert g(P, P, P, 4, 64, 3, None) == DTYPE
+    assert g(None, None, None, 0, 64, BF16, None) == OK
 
 
 def test_swiglu_argument_checks(lib):  # noqa: F811
@@ -167,8 +165,6 @@ def test_binding_refuses_what_the_library_cannot_see(emulated):  # noqa: F811
                 lambda: _C.mx8_quantize(x, codes.to(torch.uint8), scales), lambda: _C.mx8_quantize(x, codes, scales[:, :1]),
                 lambda: _C.mx8_quantize(x.double(), codes, scales),
                 lambda: _C.mx8_dequantize(codes, scales, x[:2]),
-                lambda: _C.mx8_dequantize(codes, scales, x, torch.zeros(3, dtype=torch.int64)),
-                lambda: _C.mx8_dequantize(codes, scales, x, torch.zeros(4, dtype=torch.int32)),
                 lambda: _C.rmsnorm_forward_mx8(x, None, None, x.clone(), None, kept[:-1], 1e-5),
                 lambda: _C.rmsnorm_forward_mx8(x, x, None, x.clone(), None, kept, 1e-5),
                 lambda: _C.rmsnorm_forward_mx8(x, None, torch.ones(63), x.clone(), None, kept, 1e-5),
