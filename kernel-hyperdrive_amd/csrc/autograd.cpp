@@ -10,6 +10,9 @@
 // points up, so that another build of it can be put in place.
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <dlfcn.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
 #include "../../include/cute_hip.h"
@@ -119,6 +122,22 @@ Tensor bytes(int64_t n, const Tensor& like, at::ScalarType type = at::kChar) {
     return at::empty({n}, like.options().dtype(type));
 }
 
+// Gradients the kernels computed know nothing of how they depend on what they came from: where a graph of the backward is
+// asked for (create_graph=True), going through them is an error instead of a gradient with a part missing.
+// (The error stands between the gradients and the operator's own inputs, so that it is met on every way to them.)
+variable_list not_differentiable(variable_list grads) {
+    const auto node = at::GradMode::is_enabled() ? torch::autograd::get_current_node() : nullptr;
+    if (node == nullptr) return grads;
+    const auto error = std::make_shared<torch::autograd::Error>(
+        "cute_kernels: the backward of this operator has no derivative of its own", torch::autograd::edge_list(node->next_edges()));
+    for (Tensor& g : grads) {
+        if (!g.defined()) continue;
+        g = g.detach();
+        torch::autograd::set_history(g, error);
+    }
+    return grads;
+}
+
 // ---- the pair --------------------------------------------------------------------------------------------------------
 std::tuple<Tensor, Tensor> mx8_quantize(const Tensor& input) {
     at::NoGradGuard no_grad;
@@ -192,7 +211,7 @@ struct SwigluMX8 : torch::autograd::Function<SwigluMX8> {
                                              dtype_code(dy.scalar_type()), stream_of(dy)),
                   "ck_swiglu_backward_mx8");
         }
-        return {gate_grad, up_grad};
+        return not_differentiable({gate_grad, up_grad});
     }
 };
 
@@ -236,7 +255,7 @@ struct SwigluUnchunkedMX8 : torch::autograd::Function<SwigluUnchunkedMX8> {
                                              dtype_code(dy.scalar_type()), stream_of(dy)),
                   "ck_swiglu_backward_mx8");
         }
-        return {x_grad};
+        return not_differentiable({x_grad});
     }
 };
 
@@ -297,7 +316,7 @@ struct RMSNormMX8 : torch::autograd::Function<RMSNormMX8> {
         const auto saved = ctx->get_saved_variables();
         const c10::DeviceGuard guard(grads[0].device());
         auto [x_grad, weight_grad] = rmsnorm_backward(saved[0], saved[1], grads[0].contiguous(), Tensor());
-        return {x_grad, weight_grad, Tensor()};
+        return not_differentiable({x_grad, weight_grad, Tensor()});
     }
 };
 
@@ -322,7 +341,7 @@ struct ResidualRMSNormMX8 : torch::autograd::Function<ResidualRMSNormMX8> {
         auto [x_grad, weight_grad] = rmsnorm_backward(saved[0], weight, grads[0].contiguous(),
                                                       grads[1].defined() ? grads[1].contiguous() : Tensor());
         // the sum hands the same gradient to both of its terms
-        return {x_grad, x_grad, weight_grad, Tensor()};
+        return not_differentiable({x_grad, x_grad, weight_grad, Tensor()});
     }
 };
 
@@ -373,7 +392,7 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
                                                logits.size(0), logits.size(1), dtype_code(logits.scalar_type()),
                                                stream_of(logits)),
               "ck_moe_balance_loss_backward");
-        return {d_logits, Tensor(), Tensor()};
+        return not_differentiable({d_logits, Tensor(), Tensor()});
     }
 };
 

@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
 }
 
 // Rows are dealt round-robin to the teams.
-// With q the codes and e the step of a block:  dx = r (dy w) - (r^3 mean(dy w s^) e) q,  dw += (dy e r) q  - the steps are
+// With q the codes and e the step of a block:  dx = r (dy w) - (r^2 mean(dy w s^) (r e)) q,  dw += (dy e r) q  - the steps are
 // folded into factors of a piece, so the kept row costs one conversion an element and no multiplication of its own.
 template <typename T, int TPR, int UNITS, bool HAS_W, bool DSUM, bool VEC>
 __global__ void __launch_bounds__(TPR > 256 ? TPR : 256, mx_bwd_residency(sizeof(typename T::storage_t), TPR))
@@ -230,7 +230,8 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256, mx_bwd_residency(sizeof
             }
         }
         dot = mx_team_sum<TPR>(dot, red[turn]);
-        const float rstd = cur.rstd, k = rstd * rstd * rstd * inv_h * dot;
+        // (the factors in this order: r^3 by itself leaves fp32's range at rows of 2^43 and of 2^-43)
+        const float rstd = cur.rstd, k = rstd * (rstd * dot) * inv_h;
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
             const int p = t + i * TPR, n = mx_piece_size<N>(H, p), at = LEAN ? 0 : i;
@@ -238,7 +239,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256, mx_bwd_residency(sizeof
                 if (LEAN) fetch_piece(row, i, 0, cur);
                 Piece<T, N> wp, o;
                 if (HAS_W) wp = LEAN ? load_piece<T, N, VEC, false>(w + p * N, n) : wv[HAS_W ? at : 0];
-                const float e = mx_step(cur.scale[at]), ke = k * e, er = e * rstd;
+                const float e = mx_step(cur.scale[at]), er = e * rstd, ke = k * er;
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
                     const float d = cur.g[at].up(j), q = mx_code(cur.c[at], j);
@@ -413,9 +414,16 @@ template <typename T, int TPR, int UNITS, bool RES, bool VEC>
 void mx_launch_fwd(hipStream_t s, const MxFwd& a) {
     typedef typename T::storage_t S;
     constexpr int block = TPR > 256 ? TPR : 256;
-    hipLaunchKernelGGL((ck::rmsnorm_fwd_mx8_kernel<T, TPR, UNITS, RES, VEC>), dim3((unsigned)ck_ceil_div(a.B, block / TPR)),
-                       dim3(block), 0, s, (const S*)a.x, (const S*)a.res, (const S*)a.w, (S*)a.y, (S*)a.res_out,
-                       (int8_t*)a.codes, (uint8_t*)a.scales, a.rstd, a.B, a.H, a.eps);
+    // a launch has fewer than 2^32 lanes: rows beyond take further ones (2^30 lanes' rows of any length are whole packets)
+    constexpr int64_t most = ((int64_t)1 << 30) / TPR;
+    const int64_t blocks = (a.H + ck::kMxBlock - 1) / ck::kMxBlock;
+    for (int64_t row = 0; row < a.B; row += most) {
+        const int64_t rows = a.B - row < most ? a.B - row : most, at = row * a.H;
+        hipLaunchKernelGGL((ck::rmsnorm_fwd_mx8_kernel<T, TPR, UNITS, RES, VEC>), dim3((unsigned)ck_ceil_div(rows, block / TPR)),
+                           dim3(block), 0, s, (const S*)a.x + at, RES ? (const S*)a.res + at : (const S*)nullptr, (const S*)a.w,
+                           (S*)a.y + at, RES ? (S*)a.res_out + at : (S*)nullptr, (int8_t*)a.codes + at,
+                           (uint8_t*)a.scales + row * blocks, a.rstd + row, rows, a.H, a.eps);
+    }
 }
 // teams of 128 and 512 lanes only where alignment lets them be fast: rows read element by element take the next wider one
 template <typename T, bool RES, bool VEC>

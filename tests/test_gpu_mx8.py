@@ -389,6 +389,42 @@ def test_rmsnorm_bad_rows_stay_alone(gpu):
     check_norm(flat[1:].view(4, 96), weight, dy[:4], None, 1e-6, y, dx, dw, dtype, "shifted")
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rmsnorm_of_far_off_rows(gpu, dtype):
+    """Rows of 2^55 and of 2^-55: their squares, and everything the results are made of, are ordinary fp32 numbers, but (1 / rms)^3
+    is not.  The bounds are those of rows of size one."""
+    from cute_kernels import rmsnorm_cute
+
+    announce("rmsnorm 8-bit far off", dtype)
+    for exponent in (55, -55):
+        for H in (72, 4104):
+            x = (randn((5, H), torch.float32, 50) * 2.0 ** exponent).to(dtype)
+            dy, weight = randn((5, H), dtype, 51), randn((H,), dtype, 52, 0.1, 1.0)
+            xg, wg = x.to(gpu, copy=True).requires_grad_(True), weight.to(gpu, copy=True).requires_grad_(True)
+            y = rmsnorm_cute(xg, wg, 0.0, checkpoint_8bit=True)
+            y.backward(dy.to(gpu))
+            check_norm(x, weight, dy, None, 0.0, y, xg.grad, wg.grad, dtype, f"2^{exponent} H={H}")
+
+
+def test_rmsnorm_of_more_rows_than_a_launch_holds(gpu):
+    """2^24 + 5 rows of 64 lanes each are more than the 2^30 lanes one launch of the forward takes."""
+    if gpu.type != "cuda":
+        pytest.skip("too many rows for the emulation")
+    from cute_kernels import rmsnorm_cute
+
+    announce("rmsnorm 8-bit many rows")
+    B, H = 2 ** 24 + 5, 40
+    x = torch.randn(B, H, dtype=torch.bfloat16, device=gpu, generator=torch.Generator(gpu).manual_seed(53)).requires_grad_(True)
+    dy = torch.randn(B, H, dtype=torch.bfloat16, device=gpu, generator=torch.Generator(gpu).manual_seed(54))
+    y = rmsnorm_cute(x, None, 1e-5, checkpoint_8bit=True)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    for rows in (slice(0, 300), slice(2 ** 24 - 300, B)):
+        part = x[rows].detach().clone().requires_grad_(True)
+        want = rmsnorm_cute(part, None, 1e-5, checkpoint_8bit=True)
+        assert torch.equal(y[rows], want)
+        assert torch.equal(dx[rows], torch.autograd.grad(want, part, dy[rows])[0])
+
+
 # ---- differences ------------------------------------------------------------------------------------------------------------
 def test_gradients_against_differences(gpu):
     """The gradients are those of the operators at the kept values.  x is made of values that are kept exactly (multiples of
@@ -680,3 +716,83 @@ def test_compiled_and_python_host_paths_agree(gpu, dtype, monkeypatch):
     finally:
         set_cute_tracing(False)
     assert len(traced) == len(eager) and all(torch.equal(a, b) for a, b in zip(eager, traced))
+
+
+def test_no_second_derivative(gpu):
+    """The gradients of the kernels say nothing about how they depend on their inputs: differentiating through them is an
+    error, also where the other terms of a sum could be differentiated."""
+    import cute_kernels as ck
+
+    announce("no second derivative")
+    x, res = randn((5, 64), torch.float32, 60).to(gpu), randn((5, 64), torch.float32, 61).to(gpu)
+    ids = torch.tensor([[0], [1], [2], [3], [4]], device=gpu)
+    calls = [
+        lambda v: ck.rmsnorm_cute(v, None, 1e-5, checkpoint_8bit=True).square().sum(),
+        lambda v: ck.fused_residual_add_rmsnorm_cute(v, res, None, 1e-5, checkpoint_8bit=True)[0].square().sum(),
+        lambda v: ck.swiglu_cute(v, res, checkpoint_8bit=True).square().sum(),
+        lambda v: ck.swiglu_unchunked_cute(v, checkpoint_8bit=True).square().sum(),
+        lambda v: ck.moe_balance_loss_cute(v, ids)[0].square(),
+    ]
+    for call in calls:
+        v = x.clone().requires_grad_(True)
+        (first,) = torch.autograd.grad(call(v), v)
+        (again,) = torch.autograd.grad(call(v), v, create_graph=True)
+        assert torch.equal(first, again.detach())
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(again.square().sum(), v)
+        if gpu.type == "cuda":
+            (again,) = torch.autograd.grad(call(v), v, create_graph=True)
+            with pytest.raises(RuntimeError, match="no derivative of its own"):
+                torch.autograd.grad((again.square() + v.pow(3)).sum(), v)
+
+
+@pytest.fixture
+def fresh_dynamo():
+    torch._dynamo.reset()
+    yield
+    torch._dynamo.reset()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_torch_compile(gpu, dtype, fresh_dynamo):
+    """Whole calls traced without a break: forward and backward the eager call's bit for bit (the same kernels)."""
+    import cute_kernels as ck
+
+    announce("8-bit under torch.compile", dtype)
+    x, res, dy = (randn((33, 136), dtype, 70 + i).to(gpu) for i in range(3))
+    weight = randn((136,), dtype, 73, 0.1, 1.0).to(gpu)
+    ids = torch.arange(66, device=gpu).view(33, 2) % 136
+
+    def norm(a, b, w):
+        return ck.rmsnorm_cute(a, w, 1e-5, checkpoint_8bit=True)
+
+    def residual(a, b, w):
+        return ck.fused_residual_add_rmsnorm_cute(a, b, w, 1e-5, checkpoint_8bit=True)
+
+    def glu(a, b, w):
+        return ck.swiglu_cute(a, b, checkpoint_8bit=True)
+
+    def unchunked(a, b, w):
+        return ck.swiglu_unchunked_cute(a, checkpoint_8bit=True)
+
+    def balance(a, b, w):
+        return ck.moe_balance_loss_cute(a, ids, None)
+
+    def pair(a, b, w):
+        codes, scales = ck.mx8_quantize_cute(a)
+        return codes, scales, ck.mx8_dequantize_cute(codes, scales, dtype)
+
+    for function in (norm, residual, glu, unchunked, balance, pair):
+        runs = []
+        for call in (function, torch.compile(function, fullgraph=True, backend="aot_eager")):
+            leaves = [t.clone().requires_grad_(True) for t in (x, res, weight)]
+            out = call(*leaves)
+            out = list(out) if isinstance(out, tuple) else [out]
+            through = [o for o in out if o.requires_grad]
+            grads = []
+            if through:
+                seeds = [dy[tuple(slice(0, n) for n in o.shape)] if o.dim() else torch.ones_like(o) for o in through]
+                grads = torch.autograd.grad(through, leaves, seeds, allow_unused=True)
+            runs.append([t.detach() for t in (*out, *grads) if t is not None])
+        assert len(runs[0]) == len(runs[1]), function.__name__
+        assert all(torch.equal(a, b) for a, b in zip(*runs)), function.__name__

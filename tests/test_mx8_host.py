@@ -260,6 +260,9 @@ for shape in [(1, 1), (4, 512), (2, 3, 1024), (3, 4104), (2, 8191)]:
     case(X.test_rmsnorm, dtype=BF, has_weight=True, shape=shape)
 case(X.test_rmsnorm, dtype=FP32, has_weight=False, shape=(3, 4104))
 case(X.test_rmsnorm_bad_rows_stay_alone)
+case(X.test_rmsnorm_of_far_off_rows, dtype=BF)
+case(X.test_rmsnorm_of_far_off_rows, dtype=FP32)
+case(X.test_no_second_derivative)
 case(X.test_gradients_against_differences)
 case(X.test_moe_layer, dtype=BF, shape=(100, 64, 128, 4, 2))
 case(X.test_compiled_and_python_host_paths_agree, dtype=BF)
