@@ -354,8 +354,9 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
                                  const std::optional<Tensor>& mask_in) {
         const Tensor mask = contiguous_or_none(mask_in);
         TORCH_CHECK(logits.is_cuda(), "cute_kernels HIP kernels need GPU tensors; got a tensor on ", logits.device());
-        TORCH_CHECK(selected.device() == logits.device() && (!mask.defined() || mask.device() == logits.device()),
-                    "tensors on different devices (", logits.device(), " and ", selected.device(), ")");
+        for (const Tensor* t : {&selected, &mask})
+            TORCH_CHECK(!t->defined() || t->device() == logits.device(), "tensors on different devices (", logits.device(),
+                        " and ", t->device(), ")");
         TORCH_CHECK_VALUE(logits.dim() == 2 && (logits.size(1) <= 1 || logits.stride(1) == 1),
                           "moe_balance_loss: logits need unit stride over the experts");
         const int64_t T = logits.size(0), E = logits.size(1);

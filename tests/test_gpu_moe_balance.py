@@ -339,3 +339,32 @@ def test_streams_and_graphs(gpu):
             torch.cuda.synchronize()
             for n in (0, 1):
                 assert all(torch.equal(a, b) for a, b in zip(statics[n][1], expected[(turn + n) % 3])), (turn, n)
+
+
+def test_offsets_beyond_32_bits(gpu):
+    """Only tokens behind the 2^32-nd logit count: the losses are those of these tokens alone.  One workgroup holds them all in
+    either call, in another order: sums of 300 terms (300 * 2^-24 of them), the gradient rounded to bf16 behind that."""
+    if gpu.type != "cuda":
+        pytest.skip("too large for the emulation")
+    from cute_kernels import moe_balance_loss_cute
+
+    announce("balance offsets")
+    T, E, k = 2 ** 22 + 1000, 1024, 2
+    logits, ids, _ = case(300, E, k, torch.bfloat16, 41, 0.0)
+    z = torch.zeros(T, E, dtype=torch.bfloat16, device=gpu)
+    z[-300:] = logits.to(gpu)
+    selected = torch.zeros(T, k, dtype=torch.int64, device=gpu)
+    selected[-300:] = ids.to(gpu)
+    mask = torch.zeros(T, dtype=torch.bool, device=gpu)
+    mask[-300:] = True
+    small = logits.to(gpu).requires_grad_(True)
+    want = moe_balance_loss_cute(small, ids.to(gpu))
+    (want_d,) = torch.autograd.grad(want[0] + want[1], small)
+    z.requires_grad_(True)
+    got = moe_balance_loss_cute(z, selected, mask)
+    (d,) = torch.autograd.grad(got[0] + got[1], z)
+    assert torch.equal(got[2], want[2])
+    for a, b in zip(got[:2], want[:2]):
+        assert abs(float(a) - float(b)) <= 300 * 2.0 ** -24 * abs(float(b))
+    # the sums reach a token's gradient through nothing but the counts: the same bits
+    assert torch.equal(d[-300:], want_d) and not d[:-300].any()

@@ -425,6 +425,38 @@ def test_rmsnorm_of_more_rows_than_a_launch_holds(gpu):
         assert torch.equal(dx[rows], torch.autograd.grad(want, part, dy[rows])[0])
 
 
+@pytest.mark.parametrize("H", [65536, 65530])
+def test_offsets_beyond_32_bits(gpu, H):
+    """Rows behind the 2^32-nd element: the same bits as the same rows in a small tensor."""
+    if gpu.type != "cuda":
+        pytest.skip("too large for the emulation")
+    import cute_kernels as ck
+
+    announce("8-bit offsets", H)
+    B, dtype = 2 ** 16 + 40, torch.bfloat16
+    x = torch.empty(B, H, dtype=dtype, device=gpu)
+    x[:-30].fill_(0.5)
+    x[-30:] = randn((30, H), dtype, 55).to(gpu)
+    x.requires_grad_(True)
+    weight, dy = randn((H,), dtype, 56, 0.1, 1.0).to(gpu), randn((30, H), dtype, 57).to(gpu)
+    tail = x[-30:].detach().clone().requires_grad_(True)
+    codes, scales = ck.mx8_quantize_cute(x)
+    want = ck.mx8_quantize_cute(tail)
+    assert torch.equal(codes[-30:], want[0]) and torch.equal(scales[-30:], want[1])
+    assert torch.equal(ck.mx8_dequantize_cute(codes, scales, dtype)[-30:], ck.mx8_dequantize_cute(*want, dtype))
+    del codes, scales
+    for call in (lambda v: ck.swiglu_unchunked_cute(v, checkpoint_8bit=True),
+                 lambda v: ck.rmsnorm_cute(v, weight, 1e-5, checkpoint_8bit=True)):
+        y, want = call(x), call(tail)
+        assert torch.equal(y[-30:], want)
+        grad = torch.zeros_like(y)
+        grad[-30:] = dy[:, : y.size(-1)]
+        (dx,) = torch.autograd.grad(y, x, grad)
+        assert torch.equal(dx[-30:], torch.autograd.grad(want, tail, dy[:, : y.size(-1)].contiguous())[0])
+        assert not dx[-2000:-30].any()
+        del y, grad, dx
+
+
 # ---- differences ------------------------------------------------------------------------------------------------------------
 def test_gradients_against_differences(gpu):
     """The gradients are those of the operators at the kept values.  x is made of values that are kept exactly (multiples of
