@@ -308,37 +308,37 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256, mx_bwd_residency(sizeof
     }
 }
 
-// dw[col] = sum of the partial rows, in a fixed order: a workgroup owns 16 columns, 64 groups of rows by 4 column quads
+// dw[col] = sum of the partial rows, in a fixed order: a workgroup owns 32 columns (a cache line of each partial row), 8 column
+// quads by 128 groups of rows.  768 partial rows of 4096: 4.3 us, and 5.6 with 16 columns, where every line is fetched twice.
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
     rmsnorm_dw_mx8_kernel(const float* __restrict__ partial, typename T::storage_t* __restrict__ dw, int parts, int H,
                           int padded) {
-    __shared__ float4 waves[4][4];
-    const int quad = threadIdx.x & 3;
-    const int col = blockIdx.x * 16 + quad * 4;
+    __shared__ float4 waves[16][8];
+    const int quad = threadIdx.x & 7;
+    const int col = blockIdx.x * 32 + quad * 4;  // (rows are padded to a multiple of 32)
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (col < padded) {
-        for (int r = threadIdx.x >> 2; r < parts; r += 64) {
-            const float4 v = *reinterpret_cast<const float4*>(partial + (int64_t)r * padded + col);
-            acc.x += v.x;
-            acc.y += v.y;
-            acc.z += v.z;
-            acc.w += v.w;
-        }
+#pragma unroll 4
+    for (int r = threadIdx.x >> 3; r < parts; r += 128) {
+        const float4 v = *reinterpret_cast<const float4*>(partial + (int64_t)r * padded + col);
+        acc.x += v.x;
+        acc.y += v.y;
+        acc.z += v.z;
+        acc.w += v.w;
     }
 #pragma unroll
-    for (int off = 4; off < CK_WAVE; off <<= 1) {
+    for (int off = 8; off < CK_WAVE; off <<= 1) {
         acc.x += __shfl_xor(acc.x, off, CK_WAVE);
         acc.y += __shfl_xor(acc.y, off, CK_WAVE);
         acc.z += __shfl_xor(acc.z, off, CK_WAVE);
         acc.w += __shfl_xor(acc.w, off, CK_WAVE);
     }
-    if (lane_id() < 4) waves[threadIdx.x / CK_WAVE][quad] = acc;
+    if (lane_id() < 8) waves[threadIdx.x / CK_WAVE][quad] = acc;
     __syncthreads();
-    if (threadIdx.x < 4) {
+    if (threadIdx.x < 8) {
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
+        for (int m = 0; m < 16; ++m) {
             const float4 v = waves[m][quad];
             sum[0] += v.x;
             sum[1] += v.y;
@@ -546,7 +546,7 @@ extern "C" int ck_rmsnorm_backward_mx8(const void* codes, const void* scales, co
         // (an empty batch still defines dweight = 0: no partial rows)
         CK_DISPATCH_DTYPE(dtype, {
             typedef typename T::storage_t S;
-            hipLaunchKernelGGL((ck::rmsnorm_dw_mx8_kernel<T>), dim3((unsigned)ck_ceil_div(H, 16)), dim3(256), 0, s,
+            hipLaunchKernelGGL((ck::rmsnorm_dw_mx8_kernel<T>), dim3((unsigned)ck_ceil_div(H, 32)), dim3(1024), 0, s,
                                (const float*)workspace, (S*)weight_grad, parts, (int)H, padded);
         });
     }
