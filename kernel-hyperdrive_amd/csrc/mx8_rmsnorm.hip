@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256, mx_bwd_residency(sizeof
 }
 
 // dw[col] = sum of the partial rows, in a fixed order: a workgroup owns 32 columns (a cache line of each partial row), 8 column
-// quads by 128 groups of rows.  768 partial rows of 4096: 4.3 us, and 5.6 with 16 columns, where every line is fetched twice.
+// quads by 128 groups of rows.  768 partial rows of 4096: 4.6 us, and 5.6 with 16 columns, where every line is fetched twice.
 template <typename T>
 __global__ void __launch_bounds__(1024)
     rmsnorm_dw_mx8_kernel(const float* __restrict__ partial, typename T::storage_t* __restrict__ dw, int parts, int H,
