@@ -164,16 +164,16 @@ class _Launch:
     __slots__ = ("index", "guard", "stream")
 
     def __init__(self, *tensors):
-        # one device number per tensor (-1: not on a GPU); anything else is looked at, and refused, by _require_gpu
-        index = -1
+        # the device number of every tensor (below zero: not on a GPU); what is not one GPU's throughout is refused by
+        # _require_gpu, which says why
+        index = None
         for t in tensors:
             if t is not None:
                 i = t.get_device()
-                if i != index:
-                    if index >= 0 or i < 0:
-                        _require_gpu(*tensors)
-                    index = i
-        if index < 0:
+                if i < 0 or (index is not None and i != index):
+                    _require_gpu(*tensors)
+                index = i
+        if index is None:
             _require_gpu(*tensors)
         self.index = index
         self.guard = None
