@@ -133,7 +133,9 @@ __device__ __forceinline__ uint64_t wave_match(uint32_t digit, int bits, bool va
 }
 
 // ---- activations ---------------------------------------------------------------------------
-// Exact-ish sigmoid for fp32 storage, fast-exp version for 16-bit storage (their rounding hides it).
+// fp32 storage: the sigmoid to a few units in its last place at every x - e / (1 + e) with e = exp(x) for x < 0 (1 minus the
+// mirrored value would lose the digits of a small result: 4e-5 of it at x = -8, all of them at -18).  16-bit storage: the
+// fast exponential and reciprocal, whose errors the rounding hides.
 template <typename T>
 __device__ __forceinline__ float sigmoidf_(float x);
 template <>
@@ -141,7 +143,7 @@ __device__ __forceinline__ float sigmoidf_<F32>(float x) {
     // evaluate on the side where exp() cannot overflow
     const float e = expf(-fabsf(x));
     const float s = 1.0f / (1.0f + e);
-    return x >= 0.f ? s : 1.0f - s;
+    return x < 0.f ? e * s : s;
 }
 // (v_rcp_f32 is good to 1 ulp of fp32, far below what a 16-bit result keeps; a correctly rounded division
 // costs ten more instructions per element, which shows where the activation runs in a GEMM epilogue)

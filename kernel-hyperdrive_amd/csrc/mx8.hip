@@ -135,18 +135,6 @@ __global__ void __launch_bounds__(kMxThreads)
     }
 }
 
-// sigmoid(x) with its relative accuracy kept on both sides (for x < 0 it is the exponential itself that carries it)
-template <typename T>
-__device__ __forceinline__ float mx_sigmoid(float x) {
-    return sigmoidf_<T>(x);
-}
-template <>
-__device__ __forceinline__ float mx_sigmoid<F32>(float x) {
-    const float e = expf(-fabsf(x));
-    const float r = 1.0f / (1.0f + e);
-    return x >= 0.f ? r : e * r;
-}
-
 // ACT: also writes the activation the kept inputs give (for the next product's weight gradient)
 template <typename T, int MODE, bool ACT>
 __global__ void __launch_bounds__(kMxThreads)
@@ -168,7 +156,7 @@ __global__ void __launch_bounds__(kMxThreads)
 #pragma unroll
     for (int j = 0; j < N; ++j) {
         const float g = mx_code(gc, j) * gs, u = mx_code(uc, j) * us, dy1 = d.up(j);
-        const float s = mx_sigmoid<T>(g), gsig = g * s;
+        const float s = sigmoidf_<T>(g), gsig = g * s;
         og.put(j, dy1 * u * (s + gsig * (1.0f - s)));
         ou.put(j, dy1 * gsig);
         if (ACT) oa.put(j, u * gsig);

@@ -1,0 +1,28 @@
+"""Further GPU test bodies of the 8-bit checkpoints, the balance loss and the operators they share code with, on the CPU
+emulation of the kernels."""
+
+import inspect
+
+import pytest
+
+import test_gpu_swiglu_far_gates as far_gates
+from test_emulated_device import emulated, library  # noqa: F401 (fixtures)
+
+CASES = []
+
+
+def case(function, **arguments):
+    label = function.__name__[5:] + "-" + "-".join(str(v).replace("torch.", "") for v in arguments.values())
+    CASES.append(pytest.param(function, arguments, id=label[:90]))
+
+
+for checkpoint_8bit in (False, True):
+    for one_tensor in (False, True):
+        case(far_gates.test_far_gates_fp32, checkpoint_8bit=checkpoint_8bit, one_tensor=one_tensor)
+
+
+@pytest.mark.parametrize("function,arguments", CASES)
+def test_gpu_test_body_on_the_emulated_device(emulated, monkeypatch, function, arguments):  # noqa: F811
+    if "monkeypatch" in inspect.signature(function).parameters:
+        arguments = dict(arguments, monkeypatch=monkeypatch)
+    function(emulated, **arguments)
