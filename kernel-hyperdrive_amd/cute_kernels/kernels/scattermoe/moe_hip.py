@@ -284,20 +284,35 @@ class MoE_HIP(MoE_Torch):
     checkpoint_8bit = False
 
     def balance_loss(
-        self, router_logits: torch.Tensor, token_mask: torch.Tensor | None = None
+        self,
+        router_logits: torch.Tensor,
+        token_mask: torch.Tensor | None = None,
+        selected_experts: torch.Tensor | None = None,
     ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-        """``moe_balance_loss_cute`` of the logits this layer's forward returned, with the experts it selected by them;
-        ``token_mask``: one bool per token, in any shape."""
+        """``moe_balance_loss_cute`` of the logits this layer's forward returned; ``token_mask``: one bool per token, in any
+        shape.  ``selected_experts`` None: the logits go through the selection that the layer itself routes by - the kernel's,
+        equal logits in the order of their positions, or with ``fuse_router = False`` (and where the kernel does not take the
+        router's sizes) ``torch.topk``, which leaves the order of equal ones open: it repeats itself on the same logits in the
+        same layout, and a caller that has the ids at hand passes them."""
+        router_logits = router_logits.reshape(-1, self.num_experts)
         if token_mask is not None:
             token_mask = token_mask.reshape(-1)
-        return moe_balance_loss_cute(router_logits, None, token_mask, top_k=self.top_k)
+        if selected_experts is not None:
+            selected_experts = selected_experts.reshape(-1, self.top_k)
+        elif not self._selects_in_kernel():
+            with torch.no_grad():
+                selected_experts = self._get_topk(router_logits)[1]
+        return moe_balance_loss_cute(router_logits, selected_experts, token_mask, top_k=self.top_k)
 
-    def _compute_routing_weights(self, hidden_states: torch.Tensor):
-        if not (
+    def _selects_in_kernel(self) -> bool:
+        return (
             self.fuse_router
             and self.num_experts <= _C.ROUTER_MAX_EXPERTS
             and self.top_k <= min(self.num_experts, _C.ROUTER_MAX_TOP_K)
-        ):
+        )
+
+    def _compute_routing_weights(self, hidden_states: torch.Tensor):
+        if not self._selects_in_kernel():
             return super()._compute_routing_weights(hidden_states)
         if self.fuse_router_linear and getattr(self.gate, "bias", None) is None:
             return moe_router(hidden_states, self.gate.weight, self.top_k)

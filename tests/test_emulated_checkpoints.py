@@ -5,6 +5,7 @@ import inspect
 
 import pytest
 
+import test_gpu_layer_balance as layer_balance
 import test_gpu_swiglu_far_gates as far_gates
 from test_emulated_device import emulated, library  # noqa: F401 (fixtures)
 
@@ -19,6 +20,9 @@ def case(function, **arguments):
 for checkpoint_8bit in (False, True):
     for one_tensor in (False, True):
         case(far_gates.test_far_gates_fp32, checkpoint_8bit=checkpoint_8bit, one_tensor=one_tensor)
+for experts, top_k in [(8, 2), (12, 1), (40, 6), (100, 70), (66, 65)]:
+    for fuse_router in (True, False):
+        case(layer_balance.test_counts_are_those_of_the_routing, experts=experts, top_k=top_k, fuse_router=fuse_router)
 
 
 @pytest.mark.parametrize("function,arguments", CASES)
