@@ -760,7 +760,8 @@ def router_topk_softmax_forward(logits, weights, weights_f32, selected) -> None:
     lib = load_library()
     T, E = logits.shape
     k = selected.size(1)
-    if logits.stride(1) != 1:
+    # (the distance along a dimension of one element says nothing: torch leaves any number there)
+    if E > 1 and logits.stride(1) != 1:
         raise ValueError("router_topk_softmax_forward needs unit column stride for the logits")
     if weights.dtype != logits.dtype or weights_f32.dtype != torch.float32 or selected.dtype != torch.int64:
         raise ValueError("router_topk_softmax_forward: weights in the logits' dtype, weights_f32 fp32, selected int64")
@@ -769,8 +770,9 @@ def router_topk_softmax_forward(logits, weights, weights_f32, selected) -> None:
             raise ValueError("router_topk_softmax_forward: outputs must be dense [tokens, k]")
     with _Launch(logits, weights, weights_f32, selected) as L:
         _check(
-            lib.ck_router_topk_softmax_forward(_ptr(logits), logits.stride(0), _ptr(weights), _ptr(weights_f32),
-                                               _ptr(selected), T, E, k, dtype_code(logits.dtype), L.stream),
+            lib.ck_router_topk_softmax_forward(_ptr(logits), logits.stride(0) if T > 1 else E, _ptr(weights),
+                                               _ptr(weights_f32), _ptr(selected), T, E, k, dtype_code(logits.dtype),
+                                               L.stream),
             "ck_router_topk_softmax_forward",
         )
 

@@ -23,6 +23,7 @@ for checkpoint_8bit in (False, True):
 for experts, top_k in [(8, 2), (12, 1), (40, 6), (100, 70), (66, 65)]:
     for fuse_router in (True, False):
         case(layer_balance.test_counts_are_those_of_the_routing, experts=experts, top_k=top_k, fuse_router=fuse_router)
+case(layer_balance.test_one_token_and_one_expert_of_any_stride)
 
 
 @pytest.mark.parametrize("function,arguments", CASES)

@@ -51,3 +51,31 @@ def test_counts_are_those_of_the_routing(gpu, experts, top_k, fuse_router, monke
         (d,) = torch.autograd.grad(balance, router_logits, retain_graph=True)
         error = (d.cpu().double() - want[3]).abs()
         assert (error <= 2.0 ** -8 * want[3].abs() + 2.0 ** -18 * want[4]).all()  # (bf16 rounding, and the fp32 evaluation)
+
+
+def test_one_token_and_one_expert_of_any_stride(gpu):
+    """Along a dimension of one element a tensor's stride can be any number; the selection takes it as the losses do."""
+    from cute_kernels import moe_balance_loss_cute
+
+    announce("balance strides of one")
+    wide = randn((20, 8), torch.float32, 80)
+    views = [
+        (lambda t: t[:1, :5].t(), 1),  # five tokens, one expert, the next column a row away
+        (lambda t: t[:1].expand(20, 8)[:1], 2),  # one token of an expanded row: stride 0
+        (lambda t: t[0].view(8, 1).t(), 2),  # one token, stride 1
+        (lambda t: t[3:4, 2:3], 1),
+        (lambda t: t[:, 1:2], 1),
+        (lambda t: t[7], 2),
+    ]
+    for view, top_k in views:
+        z = wide.to(gpu, copy=True).requires_grad_(True)
+        logits = view(z)
+        host = view(wide).reshape(-1, logits.size(-1))
+        ids = host.topk(top_k, dim=-1).indices
+        want = reference(host, ids, None, 1.0, 1.0)
+        balance, z_loss, counts = moe_balance_loss_cute(logits, top_k=top_k)
+        assert torch.equal(counts.cpu().long(), want[2])
+        assert abs(float(balance.detach()) - float(want[0])) <= 2.0 ** -19 * float(want[0])
+        (d,) = torch.autograd.grad(balance + z_loss, logits)
+        error = (d.cpu().double().reshape(want[3].shape) - want[3]).abs()
+        assert (error <= 2.0 ** -23 * want[3].abs() + 2.0 ** -18 * want[4]).all()
