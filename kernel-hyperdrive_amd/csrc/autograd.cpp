@@ -402,6 +402,13 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     const auto unlocked = py::call_guard<py::gil_scoped_release>();
     m.def("load", &load);
+    m.def("not_differentiable", [](const std::vector<std::optional<Tensor>>& grads) {
+        variable_list given;
+        for (const auto& g : grads) given.push_back(g.value_or(Tensor()));
+        std::vector<std::optional<Tensor>> out;
+        for (const Tensor& g : not_differentiable(given)) out.push_back(g.defined() ? std::optional<Tensor>(g) : std::nullopt);
+        return out;
+    });
     m.def("mx8_quantize", &mx8_quantize, unlocked);
     m.def("mx8_dequantize", &mx8_dequantize, unlocked);
     m.def("swiglu", [](const Tensor& gate, const Tensor& up) { return SwigluMX8::apply(gate, up); }, unlocked);

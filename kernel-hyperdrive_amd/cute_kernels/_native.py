@@ -47,3 +47,14 @@ def functions_for(tensor: torch.Tensor):
     if not tensor.is_cuda or torch.compiler.is_compiling() or is_cute_tracing():
         return None
     return _module or load()
+
+
+def not_differentiable(*grads: torch.Tensor | None) -> tuple[torch.Tensor | None, ...]:
+    """For the end of a Python autograd function's backward that computes its gradients in kernels: where a graph of the
+    backward is asked for (``create_graph=True``), differentiating them again is an error on every way to the function's
+    inputs.  (torch's ``once_differentiable`` puts its error beside those ways: a sum of which another term can be
+    differentiated misses this one without a word.)  While a graph is traced torch.compile itself refuses a second
+    derivative."""
+    if torch.compiler.is_compiling() or not torch.is_grad_enabled():
+        return grads
+    return tuple(load().not_differentiable(list(grads)))

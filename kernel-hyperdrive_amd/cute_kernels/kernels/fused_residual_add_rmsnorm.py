@@ -149,7 +149,7 @@ class _FusedResidualAddRMSNormMX8_Cute(torch.autograd.Function):
             return residual_output_grad, residual_output_grad, None if weight is None else torch.zeros_like(weight), None
         x_grad, weight_grad = rmsnorm_backward_mx8(ctx.saved_tensors, output_grad, residual_output_grad)
         # the sum hands the same gradient to both of its terms
-        return x_grad, x_grad, weight_grad, None
+        return _native.not_differentiable(x_grad, x_grad, weight_grad, None)
 
 
 def fused_residual_add_rmsnorm_cute(

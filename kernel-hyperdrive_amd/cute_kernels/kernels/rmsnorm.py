@@ -316,7 +316,7 @@ class _RMSNormMX8_Cute(torch.autograd.Function):
     @staticmethod
     def backward(ctx, output_grad: torch.Tensor):
         x_grad, weight_grad = rmsnorm_backward_mx8(ctx.saved_tensors, output_grad, None)
-        return x_grad, weight_grad, None
+        return _native.not_differentiable(x_grad, weight_grad, None)
 
 
 def rmsnorm_cute(

@@ -83,7 +83,7 @@ class _MoEBalanceLoss_Cute(torch.autograd.Function):
             return None, None, None
         d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         moe_balance_loss_backward_hip(logits, mask, shares, balance_grad, z_grad, d_logits)
-        return d_logits, None, None
+        return _native.not_differentiable(d_logits, None, None)
 
 
 def moe_balance_loss_cute(

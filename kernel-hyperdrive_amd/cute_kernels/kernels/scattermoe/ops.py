@@ -27,7 +27,7 @@ import os
 
 import torch
 
-from ... import _C
+from ... import _C, _native
 from ...constants import LIBRARY_NAME
 from ...cutotune import CutoTuneConfig, CutoTuneParameter, cutotune, get_cartesian_product_cutotune_configs
 from ...utils import cute_op
@@ -626,7 +626,7 @@ class _ScatteredGLUExpertsMX8(torch.autograd.Function):
         )
         d_input = _sum_over_slots(d_expanded_input, x.size(0), k)
         # x, w_fc, w_proj, k, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates
-        return d_input, d_w_fc, d_w_proj, None, None, None, None, d_gates
+        return _native.not_differentiable(d_input, d_w_fc, d_w_proj, None, None, None, None, d_gates)
 
 
 def scattered_glu_experts(

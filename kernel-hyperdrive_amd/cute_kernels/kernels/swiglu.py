@@ -128,7 +128,7 @@ class _SwigluMX8_Cute(torch.autograd.Function):
         gate_grad = torch.empty_like(output_grad)
         up_grad = torch.empty_like(output_grad)
         swiglu_backward_mx8_hip(ctx.saved_tensors[0], output_grad, gate_grad, up_grad)
-        return gate_grad, up_grad
+        return _native.not_differentiable(gate_grad, up_grad)
 
 
 def swiglu_cute(

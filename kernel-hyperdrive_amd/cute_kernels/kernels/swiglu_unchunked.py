@@ -130,7 +130,7 @@ class _SwigluUnchunkedMX8_Cute(torch.autograd.Function):
         *lead, h = output_grad.shape
         x_grad = torch.empty((*lead, 2 * h), device=output_grad.device, dtype=output_grad.dtype)
         swiglu_unchunked_backward_mx8_hip(ctx.saved_tensors[0], output_grad, x_grad, None)
-        return x_grad
+        return _native.not_differentiable(x_grad)[0]
 
 
 def swiglu_unchunked_cute(

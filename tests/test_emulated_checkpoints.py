@@ -6,6 +6,7 @@ import inspect
 import pytest
 
 import test_gpu_layer_balance as layer_balance
+import test_gpu_second_derivatives as second
 import test_gpu_swiglu_far_gates as far_gates
 from test_emulated_device import emulated, library  # noqa: F401 (fixtures)
 
@@ -24,6 +25,10 @@ for experts, top_k in [(8, 2), (12, 1), (40, 6), (100, 70), (66, 65)]:
     for fuse_router in (True, False):
         case(layer_balance.test_counts_are_those_of_the_routing, experts=experts, top_k=top_k, fuse_router=fuse_router)
 case(layer_balance.test_one_token_and_one_expert_of_any_stride)
+for name in ("rmsnorm", "residual", "residual-both", "swiglu", "unchunked", "balance", "z-loss"):
+    for path in ("python", "traced"):
+        case(second.test_operators, name=name, path=path)
+case(second.test_layer)
 
 
 @pytest.mark.parametrize("function,arguments", CASES)
