@@ -362,8 +362,8 @@ int ck_moe_balance_loss_backward(const void* logits, int64_t ld, const void* mas
  * Activations kept in 8 bits between forward and backward (no counterpart in the reference): MXINT8 of the OCP
  * microscaling formats.  A block is 32 consecutive elements of a row, the last one of a row may be shorter; it has one
  * scale byte b and int8 codes q in [-127, 127], element = q * 2^(b - 133).  b is the smallest exponent (7 .. 254) for
- * which the block's largest magnitude rounds to at most 127 steps; rounding is to nearest, ties to even; b = 255 marks a
- * block with a NaN or an infinity, which stands for NaNs.
+ * which the block's largest magnitude rounds to at most 127 steps (smaller ones are read, not written); rounding is to
+ * nearest, ties to even; b = 255 marks a block with a NaN or an infinity, which stands for NaNs.
  *   codes: H bytes a row, scales: ceil(H / 32) bytes a row (dense unless a stride is passed)
  * ck_mx8_quantize    x [rows, H] -> codes, scales
  * ck_mx8_dequantize  codes, scales -> output [rows, H].  A value beyond fp16's range becomes its largest finite number.

@@ -4,11 +4,11 @@
 // int8 code q in [-127, 127] per element; the element stands for  q * 2^(b - 133)  (the format's element step 2^-6 times
 // its scale 2^(b - 127)).  b is the smallest exponent for which the block's largest magnitude rounds to at most 127
 // steps: with u the bits of that magnitude as an fp32,  b = (u + 0x10000) >> 23  - the addend carries into the exponent
-// exactly when the mantissa is 255/128 or more, i.e. 127.5 steps.  b is at least 7 (steps are normal fp32 numbers) and at
-// most 254; 255 marks a block that holds a NaN or an infinity and stands for 32 NaNs.
+// exactly when the mantissa is 255/128 or more, i.e. 127.5 steps.  A written b is at least 7 (steps are normal fp32 numbers) and at
+// most 254, smaller ones are read as well; 255 marks a block that holds a NaN or an infinity and stands for 32 NaNs.
 // Scaling by a power of two is exact, so the only rounding is the one to whole steps (to nearest, ties to even: half a
 // step, 1/254 .. 1/127 of the block's largest magnitude), codes depend on nothing but the values, and q * 2^(b - 133) has seven
-// magnitude bits: it is exact in fp32 and bf16, and in fp16 up to that type's range.
+// magnitude bits: it is exact in fp32 and bf16, and in fp16 between that type's subnormal numbers and its largest.
 //
 // A lane holds one 16-byte packet of a block ("a piece"): eight elements of a 16-bit type, four of fp32, with as many bytes of
 // codes.  So four or eight neighbouring lanes hold a block, every load and store of a wave is one run of memory, and the
@@ -124,9 +124,10 @@ __device__ __forceinline__ MxCodes<N> mx_encode(const float (&values)[N], uint32
     return c;
 }
 
-// the step a scale byte stands for; NaN for 255
+// the step 2^(scale - 133) a scale byte stands for; NaN for 255.  mx_encode writes none below 7, whose steps are subnormal
+// numbers (2^-127 .. 2^-133, exact as well), but codes and scales can come from elsewhere.
 __device__ __forceinline__ float mx_step(uint32_t scale) {
-    return mx_float(scale >= 255u ? 0x7fc00000u : ((scale < 7u ? 7u : scale) - 6u) << 23);
+    return mx_float(scale >= 255u ? 0x7fc00000u : (scale < 7u ? 1u << (scale + 16u) : (scale - 6u) << 23));
 }
 // the codes as numbers (one conversion each, the byte picked and sign-extended on the way), and the values they stand for
 template <int N>

@@ -1,8 +1,8 @@
 """Activations in 8 bits: MXINT8 of the OCP microscaling formats, for what a training step keeps between forward and backward.
 
 A block is 32 consecutive elements of a row (the last one of a row may be shorter).  It has one scale byte ``b`` and an int8
-code ``q`` in [-127, 127] per element, which stands for ``q * 2 ** (b - 133)``.  ``b`` is the smallest exponent (7 .. 254)
-for which the block's largest magnitude rounds to at most 127 steps, so an element is off by at most half a step: 1/254 to 1/127 of that
+code ``q`` in [-127, 127] per element, which stands for ``q * 2 ** (b - 133)``.  ``b`` is the smallest exponent (7 .. 254; smaller
+ones written elsewhere are read too) for which the block's largest magnitude rounds to at most 127 steps, so an element is off by at most half a step: 1/254 to 1/127 of that
 magnitude.  Scaling by a power of two is exact: codes depend on nothing but the values, and writing what was read
 back changes nothing.  A block with a NaN or an infinity has scale byte 255 and stands for NaNs.
 
@@ -37,8 +37,10 @@ def mx8_quantize_torch(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 def mx8_dequantize_torch(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     H = codes.size(-1)
-    exponent = scales.to(torch.int32).clamp(min=7)
-    steps = torch.where(exponent == 255, float("nan"), ((exponent - 6) << 23).view(torch.float32))
+    exponent = scales.to(torch.int32)
+    # 2 ** (exponent - 133): below 7 a subnormal number, one bit of the mantissa
+    bits = torch.where(exponent < 7, 1 << (exponent.clamp(max=6) + 16), (exponent.clamp(min=7) - 6) << 23)
+    steps = torch.where(exponent == 255, float("nan"), bits.to(torch.int32).view(torch.float32))
     x = codes.float() * steps.repeat_interleave(_C.MX8_BLOCK, dim=-1)[..., :H]
     if dtype == torch.float16:
         x = x.clamp(-65504.0, 65504.0)
@@ -95,7 +97,8 @@ def mx8_quantize_cute(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 
 def mx8_dequantize_cute(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    """The values ``(codes, scales)`` stand for, exact in ``dtype`` (beyond float16's range: its largest finite number)."""
+    """The values ``(codes, scales)`` stand for: exact in float32 and bfloat16, rounded to float16 where they lie among its
+    subnormal numbers (beyond its range: its largest finite number)."""
     functions = _native.functions_for(codes)
     if functions is not None:
         return functions.mx8_dequantize(codes, scales, dtype)

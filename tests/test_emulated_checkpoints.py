@@ -4,8 +4,10 @@ emulation of the kernels."""
 import inspect
 
 import pytest
+import torch
 
 import test_gpu_layer_balance as layer_balance
+import test_gpu_mx8_scales as small_scales
 import test_gpu_second_derivatives as second
 import test_gpu_swiglu_far_gates as far_gates
 from test_emulated_device import emulated, library  # noqa: F401 (fixtures)
@@ -29,6 +31,10 @@ for name in ("rmsnorm", "residual", "residual-both", "swiglu", "unchunked", "bal
     for path in ("python", "traced"):
         case(second.test_operators, name=name, path=path)
 case(second.test_layer)
+for dtype in (torch.float32, torch.float16, torch.bfloat16):
+    for width in (32, 35):
+        case(small_scales.test_all_scale_bytes, dtype=dtype, width=width)
+case(small_scales.test_products_of_small_blocks)
 
 
 @pytest.mark.parametrize("function,arguments", CASES)
