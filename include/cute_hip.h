@@ -38,7 +38,8 @@ typedef enum {
 
 /* Human-readable text for a ck_status (host pointer to a static string). */
 const char* ck_status_string(int status);
-/* Library version, bumped when a signature changes. */
+/* Version of the signatures below, bumped when one changes: what a caller was compiled against, and what the library is. */
+#define CK_ABI_VERSION 3
 int ck_abi_version(void);
 
 /* ---------------------------------------------------------------------------------------------

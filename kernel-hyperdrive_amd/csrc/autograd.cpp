@@ -401,6 +401,8 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     const auto unlocked = py::call_guard<py::gil_scoped_release>();
+    // the signatures this module was compiled with: `load` casts the library's entry points to them
+    m.attr("abi_version") = CK_ABI_VERSION;
     m.def("load", &load);
     m.def("not_differentiable", [](const std::vector<std::optional<Tensor>>& grads) {
         variable_list given;

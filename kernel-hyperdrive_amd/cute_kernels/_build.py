@@ -71,7 +71,7 @@ def build_autograd(verbose: bool = False) -> str:
     compiler = shutil.which("g++") or shutil.which("c++")
     if compiler is None:
         raise RuntimeError("no host C++ compiler: the host path of cute_kernels cannot be built")
-    tmp = AUTOGRAD_PATH + ".tmp"
+    tmp = f"{AUTOGRAD_PATH}.{os.getpid()}.tmp"  # (processes that import first at the same time each write their own)
     cmd = [compiler, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
            "-DTORCH_EXTENSION_NAME=cute_autograd", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
     cmd += [f"-I{path}" for path in include_paths("cuda")] + [f"-I{sysconfig.get_paths()['include']}"]
@@ -98,7 +98,7 @@ def build(verbose: bool = False, jobs: int | None = None) -> str:
         autograd = pool.submit(build_autograd, verbose)
         objects = list(pool.map(lambda src: _compile(hipcc, src, obj_dir, verbose), SOURCES))
         autograd.result()
-    tmp = LIB_PATH + ".tmp"
+    tmp = f"{LIB_PATH}.{os.getpid()}.tmp"
     link = subprocess.run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", *objects, "-o", tmp],
                           capture_output=True, text=True)
     if link.returncode != 0:

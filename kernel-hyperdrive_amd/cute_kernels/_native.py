@@ -22,6 +22,13 @@ _module = None
 _lock = threading.Lock()
 
 
+def _import(path: str):
+    spec = importlib.util.spec_from_file_location(_MODULE, path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
 def load():
     """Import (building first if nothing is built) and connect it to the kernel library; errors are not hidden."""
     global _module
@@ -35,9 +42,13 @@ def load():
         if not os.path.exists(_build.AUTOGRAD_PATH):
             _build.build_autograd()
         _C.load_library()
-        spec = importlib.util.spec_from_file_location(_MODULE, _build.AUTOGRAD_PATH)
-        module = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(module)
+        module = _import(_build.AUTOGRAD_PATH)
+        # (the library's version says nothing of the signatures an older build of the module calls it with)
+        built_for = getattr(module, "abi_version", None)
+        if built_for != _C._ABI_VERSION:
+            raise RuntimeError(
+                f"cute_autograd.so was built for ABI version {built_for}, this package needs {_C._ABI_VERSION}: rebuild it"
+            )
         module.load(_C.library_path(), _C._ABI_VERSION)
         _module = module
     return _module
