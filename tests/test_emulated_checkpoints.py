@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import test_gpu_layer_balance as layer_balance
+import test_gpu_layer_edges as edges
 import test_gpu_mx8_routing as routing
 import test_gpu_mx8_scales as small_scales
 import test_gpu_second_derivatives as second
@@ -39,6 +40,9 @@ case(small_scales.test_products_of_small_blocks)
 for dtype in (torch.float32, torch.float16, torch.bfloat16):
     case(routing.test_routing_gradients, dtype=dtype, shape=(100, 64, 128, 4, 2))
 case(routing.test_routing_gradients, dtype=torch.bfloat16, shape=(96, 72, 40, 5, 3))
+for dtype in (torch.float32, torch.bfloat16):
+    for checkpoint_8bit in (False, True):
+        case(edges.test_no_tokens, dtype=dtype, checkpoint_8bit=checkpoint_8bit)
 
 
 @pytest.mark.parametrize("function,arguments", CASES)
