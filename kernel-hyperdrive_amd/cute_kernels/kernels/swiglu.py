@@ -145,6 +145,8 @@ def swiglu_cute(
     if checkpoint_8bit and torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad):
         assert gate.shape == up.shape, "tensors gate and up should have same shape"
         assert gate.dtype == up.dtype, "tensors gate and up should have same dtype"
+        if gate.dim() == 0:
+            raise ValueError("checkpoint_8bit keeps rows: gate and up need at least one dimension")
         functions = _native.functions_for(gate)
         return _SwigluMX8_Cute.apply(gate, up) if functions is None else functions.swiglu(gate, up)
     return _Swiglu_Cute.apply(

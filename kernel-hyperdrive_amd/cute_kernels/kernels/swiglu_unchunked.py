@@ -146,6 +146,7 @@ def swiglu_unchunked_cute(
     """``checkpoint_8bit``: keep x for the backward in 8 bits (see mx8.py); the output is that of the exact x, the gradient
     that at the kept values.  The other tunables have no meaning there."""
     if checkpoint_8bit and torch.is_grad_enabled() and x.requires_grad:
+        divide_if_divisible(x.size(-1), 2, "last dimension of x must be even")
         functions = _native.functions_for(x)
         return _SwigluUnchunkedMX8_Cute.apply(x) if functions is None else functions.swiglu_unchunked(x)
     return _SwigluUnchunked_Cute.apply(

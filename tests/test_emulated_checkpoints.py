@@ -43,6 +43,7 @@ case(routing.test_routing_gradients, dtype=torch.bfloat16, shape=(96, 72, 40, 5,
 for dtype in (torch.float32, torch.bfloat16):
     for checkpoint_8bit in (False, True):
         case(edges.test_no_tokens, dtype=dtype, checkpoint_8bit=checkpoint_8bit)
+case(edges.test_refusals_are_those_of_the_ordinary_call)
 
 
 @pytest.mark.parametrize("function,arguments", CASES)

@@ -29,3 +29,25 @@ def test_no_tokens(gpu, dtype, checkpoint_8bit):
                 (y.sum() + balance).backward()
             assert y.shape == (0, H) and v.grad.shape == (0, H) and not counts.any()
             assert all(not p.grad.any() for p in moe.parameters())
+
+
+def test_refusals_are_those_of_the_ordinary_call(gpu):
+    """Odd rows of a one-tensor SwiGLU and tensors without a dimension, with and without the checkpoint, traced and eager."""
+    import cute_kernels as ck
+    from cute_kernels.utils import set_cute_tracing
+
+    announce("refusals of the checkpoints")
+    odd = torch.randn(4, 63, device=gpu, requires_grad=True)
+    scalar = torch.tensor(1.0, device=gpu, requires_grad=True)
+    for tracing in (False, True):
+        set_cute_tracing(tracing)
+        try:
+            for checkpoint_8bit in (False, True):
+                with pytest.raises(AssertionError, match="even"):
+                    ck.swiglu_unchunked_cute(odd, checkpoint_8bit=checkpoint_8bit)
+                with pytest.raises(IndexError):
+                    ck.rmsnorm_cute(scalar, None, 1e-5, checkpoint_8bit=checkpoint_8bit)
+            with pytest.raises(ValueError, match="one dimension"):
+                ck.swiglu_cute(scalar, scalar.detach(), checkpoint_8bit=True)
+        finally:
+            set_cute_tracing(False)
