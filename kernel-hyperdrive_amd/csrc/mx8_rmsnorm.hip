@@ -3,7 +3,7 @@
 //             (and s itself with a residual)
 //   backward: with s^ the kept row:  dx = r (dy w - s^ r^2 mean(dy w s^)) (+ the sum's own gradient),  dw = sum dy s^ r
 // The row (forward: as read; backward: codes and dy) stays in the registers of a team of TPR lanes, so it is read once;
-// row sums are wave64 shuffles, wider teams meet through LDS.  Lane t holds the 16-byte pieces t, t + TPR, ..: neighbouring
+// row sums are register exchanges, wider teams meet through LDS.  Lane t holds the 16-byte pieces t, t + TPR, ..: neighbouring
 // lanes hold a block.  Backward: every team walks rows and keeps its share of dw in
 // fp32 registers; a workgroup writes one partial row, a second launch adds the partial rows up.  No atomics.
 #include "ck_mx8.h"
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256, mx_bwd_residency(sizeof
 #pragma unroll
                 for (int j = 0; j < N; ++j)
                     part += (HAS_W ? cur.g[at].up(j) * wp.up(j) : cur.g[at].up(j)) * mx_code(cur.c[at], j);
-                dot += part * mx_step(cur.scale[at]);
+                dot += part * mx_step_kept(cur.scale[at]);
             }
             __builtin_amdgcn_sched_barrier(0);  // one piece at a time: widened values do not pile up in registers
         }
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256, mx_bwd_residency(sizeof
                 if (LEAN) fetch_piece(row, i, 0, cur);
                 Piece<T, N> wp, o;
                 if (HAS_W) wp = LEAN ? load_piece<T, N, VEC, false>(w + p * N, n) : wv[HAS_W ? at : 0];
-                const float e = mx_step(cur.scale[at]), er = e * rstd, ke = k * er;
+                const float e = mx_step_kept(cur.scale[at]), er = e * rstd, ke = k * er;
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
                     const float d = cur.g[at].up(j), q = mx_code(cur.c[at], j);
