@@ -96,10 +96,10 @@ def moe_balance_loss_cute(
     float16 or bfloat16, E <= 1024).
 
     ``selected_experts [..., k]``: the experts each token went to (an id outside [0, E), a dropped slot, counts nowhere); None:
-    the ``top_k`` largest logits, equal ones in the order of their positions, as the layer's router selects them.
+    the ``top_k`` (at most 64) largest logits, equal ones in the order of their positions, as the layer's router selects them.
     ``token_mask [...]`` bool: False for padding, which takes no part whatever its logits and ids hold.  Without a counting
-    token both losses are 0.  A token whose logits are all -inf or the type's lowest value has no probabilities: it counts in N
-    and adds nothing."""
+    token both losses are 0.  A token whose logits are all -inf or the type's lowest value has no probabilities and no
+    log-sum-exp: it counts in N, and its selections in the counts."""
     E = router_logits.size(-1)
     logits = router_logits if router_logits.dim() == 2 else router_logits.reshape(-1, E)
     if (E > 1 and logits.stride(1) != 1) or (logits.size(0) > 1 and logits.stride(0) < E):

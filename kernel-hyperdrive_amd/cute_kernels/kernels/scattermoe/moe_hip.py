@@ -278,8 +278,9 @@ class MoE_HIP(MoE_Torch):
     # False keeps ``self.gate`` as a module call.
     fuse_router_linear = True
     # Save the intermediate rows the experts' backward needs in 8 bits (see kernels/mx8.py): at 8192 tokens of 4096, 8 experts
-    # of 14336 and top-2 0.62 GB per call are held for the backward instead of 1.61, and a step takes 14.95 ms instead of
-    # 14.5.  Outputs stay the same, gradients are those at the kept values (bf16, that shape: 0.9-1.2 % away norm-wise).
+    # of 14336 and top-2 0.62 GB per call are held for the backward instead of 1.61, and a step (with the balance loss) takes
+    # 14.4 ms instead of 14.1.  Outputs stay the same, gradients are those at the kept values (bf16, that shape: 0.9-1.2 % away
+    # norm-wise).
     # Needs a SwiGLU between the expert products and no expert bias.
     checkpoint_8bit = False
 
