@@ -133,9 +133,9 @@ __device__ __forceinline__ uint64_t wave_match(uint32_t digit, int bits, bool va
 }
 
 // ---- activations ---------------------------------------------------------------------------
-// fp32 storage: the sigmoid to a few units in its last place at every x - e / (1 + e) with e = exp(x) for x < 0 (1 minus the
-// mirrored value would lose the digits of a small result: 4e-5 of it at x = -8, all of them at -18).  16-bit storage: the
-// fast exponential and reciprocal, whose errors the rounding hides.
+// fp32 storage: the sigmoid to a few units in its last place, down to x = -87 where it leaves the normal numbers - e / (1 + e)
+// with e = exp(x) for x < 0 (1 minus the mirrored value would lose the digits of a small result: 4e-5 of it at x = -8, all
+// of them at -18).  16-bit storage: the fast exponential and reciprocal, whose errors the rounding hides.
 template <typename T>
 __device__ __forceinline__ float sigmoidf_(float x);
 template <>
